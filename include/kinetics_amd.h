@@ -87,7 +87,9 @@ enum kin_status {
  * elements, in kin_rms_norm.  3.2.0: head_dim 64 in the token-granular
  * policies, pages of 128 tokens, teams (the fused step) or a launch of their
  * own (the token-granular policies) for the lists that a batch has beyond a
- * multiple of 256. */
+ * multiple of 256.  3.3.0: attention of a chunk of new tokens, the weight that
+ * cached tokens received from it, eviction by that weight, and the q/k norm +
+ * split with rotary positions. */
 int kin_version(void);
 
 /* Human-readable text of the last non-OK status on the calling thread
@@ -712,6 +714,129 @@ int kin_blocktopk_decode_step_f16(const kin_f16_t* q, const kin_f16_t* k, const 
                                   const int32_t* slot_ids, int num_slots, int32_t* slot_lens,
                                   kin_stream_t stream);
 
+/* ---- chunks of new tokens ---------------------------------------------------
+ * A ragged batch: sequence b brings the rows q_indptr[b] .. q_indptr[b+1]-1 of
+ * q[nnz, num_q_heads, head_dim] (q_indptr: int32 [batch+1], on the device,
+ * ascending; a sequence may bring none).  Their keys and values are already in
+ * the cache: the page table describes it AFTER the append, so with L tokens in
+ * the sequence (behind first_page_offset padding slots) and n rows, row i stands
+ * at position p = L - n + i.  It sees token j when
+ *   j < prefix_lens[b]   or   ( j <= p  and  (window == 0  or  p - j < window) ),
+ * i.e. causally, over the newest `window` tokens only if a window is given, and
+ * always the whole prefix (int32 [batch] or NULL), also the part in front of it:
+ * a prompt part that sees itself in both directions, or pinned first tokens
+ * beside a window.  Its score, for query head g,
+ *   s = sm_scale * q.k   (sm_scale 0: 1/sqrt(head_dim); not negative)
+ *   s = softcap * tanh(s / softcap)        with softcap > 0
+ *   s = s - slopes[g] * |p - j|            with slopes != NULL (fp32 [num_q_heads])
+ * Distances count the tokens that are in the cache.
+ *
+ * max_pages_per_seq: the longest page list, for planning only (a smaller number
+ * costs time, not tokens).  Page ids outside [0, num_pages) are never
+ * dereferenced: their tokens are seen by nobody.  Cache contents behind a
+ * sequence's last token or in its padding slots never reach a result, and a
+ * non-finite value reaches only the rows that see its token.  Rows of q that
+ * belong to no sequence are not read, and their rows of out and lse are left as
+ * they were.
+ */
+
+/* Bytes of workspace for kin_paged_chunk_attention (0: none needed).
+ * num_splits 0: the library's own choice of spans, as in the call. */
+size_t kin_chunk_workspace_bytes(int64_t nnz, int batch, int num_q_heads, int num_kv_heads,
+                                 int max_pages_per_seq, int page_size, int head_dim,
+                                 int num_splits);
+
+/*
+ * Attention of the chunk (the prefill that LiteSys runs through
+ * flashinfer.single_prefill_with_kv_cache, one request at a time;
+ * ref: LiteSys/litesys/attention/batch_cache.py:112-145), any mix of single
+ * tokens and prompts in one call:
+ *   out[r, g, :] = sum_j softmax_j(s)[j] * v_j,   lse[r, g] = log sum_j exp(s_j)
+ * over the seen tokens; a row that sees none gives zeros and -inf.  lse (fp32
+ * [nnz, num_q_heads], natural logarithm) may be NULL.  Scores, softmax and sums
+ * are fp32; weights are rounded to the cache's element type before the product
+ * with V, as the result is.  num_splits 0: chosen from the sizes.  Calls that
+ * may overlap in time need workspaces of their own.
+ */
+int kin_paged_chunk_attention(const kin_bf16_t* q, const kin_bf16_t* kv_cache, const int32_t* q_indptr,
+                              const int32_t* page_indices, const int32_t* page_indptr,
+                              const int32_t* last_page_len, const float* slopes,
+                              const int32_t* prefix_lens, kin_bf16_t* out, float* lse,
+                              void* workspace, size_t workspace_bytes, int64_t nnz, int batch,
+                              int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                              int64_t num_pages, int max_pages_per_seq, int first_page_offset,
+                              float sm_scale, float softcap, int window, int num_splits,
+                              kin_stream_t stream);
+int kin_paged_chunk_attention_f16(const kin_f16_t* q, const kin_f16_t* kv_cache, const int32_t* q_indptr,
+                                  const int32_t* page_indices, const int32_t* page_indptr,
+                                  const int32_t* last_page_len, const float* slopes,
+                                  const int32_t* prefix_lens, kin_f16_t* out, float* lse,
+                                  void* workspace, size_t workspace_bytes, int64_t nnz, int batch,
+                                  int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                                  int64_t num_pages, int max_pages_per_seq, int first_page_offset,
+                                  float sm_scale, float softcap, int window, int num_splits,
+                                  kin_stream_t stream);
+
+/*
+ * The weight every cached token received from the chunk, added to what it has:
+ *   scores[b, h, j] += sum over the rows p of the sequence and the query heads g
+ *                      of KV head h that see token j of exp(s_pgj - lse[p, g])
+ * with the lse that kin_paged_chunk_attention (or any attention of this library,
+ * for single tokens) wrote for the same scores; rows with lse -inf give nothing.
+ * scores: fp32 [score_blocks, num_kv_heads, score_stride], entry j of a row
+ * belonging to token j.  slot_ids (int32 [batch] or NULL): sequence b's row block
+ * is slot_ids[b] instead of b, as for kbar.  A sequence that brings no rows, is
+ * longer than score_stride or has an id outside [0, score_blocks) is left
+ * as it was, and so is everything behind a sequence's last token.  Two sequences
+ * of one call must not share a row block.  To weigh the last rows of a prompt only, pass
+ * only those rows.
+ */
+int kin_attention_mass(const kin_bf16_t* q, const kin_bf16_t* kv_cache, const float* lse, float* scores,
+                       const int32_t* q_indptr, const int32_t* page_indices, const int32_t* page_indptr,
+                       const int32_t* last_page_len, const float* slopes, const int32_t* prefix_lens,
+                       int64_t nnz, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                       int page_size, int64_t num_pages, int max_pages_per_seq, int first_page_offset,
+                       float sm_scale, float softcap, int window, int score_blocks, int score_stride,
+                       const int32_t* slot_ids, kin_stream_t stream);
+int kin_attention_mass_f16(const kin_f16_t* q, const kin_f16_t* kv_cache, const float* lse, float* scores,
+                           const int32_t* q_indptr, const int32_t* page_indices,
+                           const int32_t* page_indptr, const int32_t* last_page_len,
+                           const float* slopes, const int32_t* prefix_lens, int64_t nnz, int batch,
+                           int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                           int64_t num_pages, int max_pages_per_seq, int first_page_offset,
+                           float sm_scale, float softcap, int window, int score_blocks,
+                           int score_stride, const int32_t* slot_ids, kin_stream_t stream);
+
+/*
+ * Cuts every sequence that holds more than `budget` tokens down to it, per KV
+ * head: kept are its first sink_tokens tokens, its newest local_tokens and, of
+ * those between, the ones with the largest scores (of equal scores the lowest
+ * index; -0 equals +0, NaN is larger than everything).  The K and V rows that
+ * stay move, in their order, to tokens 0 .. budget-1 of the sequence's own pages;
+ * the rows behind them keep whatever they held.  Heads keep different tokens of
+ * a sequence but equally many.
+ *   kept      int32 [batch, num_kv_heads, budget]: the tokens that stay,
+ *             ascending, padded with -1 (a sequence within the budget: 0 .. L-1)
+ *   new_lens  int32 [batch]: min(L, budget)
+ *   scores_out  as scores (the same tensor, or one that does not overlap it):
+ *             entry i of a row becomes the score of kept[i], entries
+ *             budget .. L-1 become 0 (a sequence within the budget: a copy);
+ *             entries behind L are left as they were
+ * A sequence longer than score_stride, or with a slot id outside
+ * [0, score_blocks), keeps everything: kept is all -1, new_lens L.  The page
+ * table describes the cache before the eviction; the caller builds the new one
+ * from new_lens (pages behind it are free) and the mean keys with kin_build_kbar.
+ * The pages of a sequence must not appear twice in the table.  Rows are moved as
+ * bytes: caches of both element types.
+ */
+int kin_evict_tokens(void* kv_cache, const float* scores, float* scores_out,
+                     const int32_t* page_indices, const int32_t* page_indptr,
+                     const int32_t* last_page_len, int32_t* kept, int32_t* new_lens, int batch,
+                     int num_kv_heads, int head_dim, int page_size, int64_t num_pages,
+                     int first_page_offset, int budget, int sink_tokens, int local_tokens,
+                     int score_blocks, int score_stride, const int32_t* slot_ids,
+                     kin_stream_t stream);
+
 /* ---- row-wise layer kernels around the attention path ---------------------
  * The reference's decoder layer (benchmark/blocktopk_decoder.py:187-240) calls
  * flashinfer's RMSNorm through its custom ops layer_norm and qk_norm
@@ -763,6 +888,31 @@ int kin_qkv_norm_split_f16(const void* qkv, int64_t qkv_row_stride, const void* 
                            const void* k_weight, float eps, void* q, void* k, void* v,
                            int batch, int num_q_heads, int num_kv_heads, int head_dim,
                            kin_stream_t stream);
+
+/*
+ * kin_qkv_norm_split with rotary positions: pair i of every q and k head, its
+ * elements i and i + D/2 (D = head_dim), is turned by
+ *   angle = positions[axis[i], b] * frequency[i]
+ *   (lo, hi) -> (lo cos - hi sin, hi cos + lo sin)
+ * (the rotation LiteSys applies, ref: LiteSys/litesys/models/model_utils.py:17-52),
+ * after the norm and without a rounding between the two; one rounding at the end.
+ * positions: int32 [num_axes, tokens] (text has one axis, images and video have
+ * time, height and width); axis: int32 [D/2], which axis turns pair i (an entry
+ * outside [0, num_axes) leaves the pair as it is); freq: int64 [D/2], turns per
+ * position as a fraction of 2^64, i.e. round(frequency[i] / (2 pi) * 2^64)
+ * modulo 2^64: position times fraction is the angle modulo a turn, exactly, for every int32
+ * position.  q_weight and k_weight both NULL: no norm.
+ */
+int kin_qkv_norm_rope_split(const void* qkv, int64_t qkv_row_stride, const void* q_weight,
+                            const void* k_weight, float eps, const int32_t* positions, int num_axes,
+                            const int64_t* freq, const int32_t* axis, void* q, void* k, void* v,
+                            int tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                            kin_stream_t stream);
+int kin_qkv_norm_rope_split_f16(const void* qkv, int64_t qkv_row_stride, const void* q_weight,
+                                const void* k_weight, float eps, const int32_t* positions,
+                                int num_axes, const int64_t* freq, const int32_t* axis, void* q,
+                                void* k, void* v, int tokens, int num_q_heads, int num_kv_heads,
+                                int head_dim, kin_stream_t stream);
 
 #define KIN_ACT_SILU 0
 #define KIN_ACT_GELU 1 /* erf form */

@@ -89,12 +89,32 @@ SIGNATURES = {
     "kin_rms_norm": (c_int, [_P, _P, _P, _P, c_int64, c_int, c_int64, c_int64, c_float, _P]),
     "kin_qkv_norm_split": (c_int, [_P, c_int64, _P, _P, c_float, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),
     "kin_gated_act": (c_int, [_P, _P, _P, c_int64, c_int, c_int64, c_int64, c_int, _P]),
+    "kin_chunk_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "kin_paged_chunk_attention": (
+        c_int,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_size_t, c_int64, c_int, c_int, c_int, c_int, c_int, c_int64, c_int,
+         c_int, c_float, c_float, c_int, c_int, _P],
+    ),
+    "kin_attention_mass": (
+        c_int,
+        [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int, c_int64, c_int, c_int, c_float,
+         c_float, c_int, c_int, c_int, _P, _P],
+    ),
+    "kin_evict_tokens": (
+        c_int,
+        [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, _P, _P],
+    ),
+    "kin_qkv_norm_rope_split": (
+        c_int,
+        [_P, c_int64, _P, _P, c_float, _P, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P],
+    ),
 }
 
 # the float16 twins have the signatures of their bfloat16 originals
 for _name in ("kin_append_paged_kv", "kin_build_kbar", "kin_append_paged_kv_ragged", "kin_block_score_topk",
               "kin_sparse_paged_decode", "kin_dense_paged_decode", "kin_blocktopk_decode_step", "kin_rms_norm",
-              "kin_qkv_norm_split", "kin_gated_act", "kin_token_topk_decode", "kin_strided_topk_decode"):
+              "kin_qkv_norm_split", "kin_gated_act", "kin_token_topk_decode", "kin_strided_topk_decode",
+              "kin_paged_chunk_attention", "kin_attention_mass", "kin_qkv_norm_rope_split"):
     SIGNATURES[_name + "_f16"] = SIGNATURES[_name]
 
 _lib = None

@@ -22,7 +22,7 @@ OBJ_DIR = PKG_DIR / "build"
 PHASES_LIB_PATH = PKG_DIR / "libkinetics_amd_phases.so"
 
 SOURCES = ["kin_api.hip", "kin_append.hip", "kin_score_topk.hip", "kin_decode.hip", "kin_step.hip", "kin_token_topk.hip", "kin_token_topk_small.hip",
-           "kin_table.hip", "kin_layer.hip"]
+           "kin_table.hip", "kin_layer.hip", "kin_rope.hip", "kin_chunk.hip", "kin_mass.hip", "kin_evict.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -1,0 +1,151 @@
+// What the operators over a chunk of new tokens share (attention of the chunk, and the weight
+// every cached token received from it): the ragged batch, which tokens a row sees, and the form
+// of the scores.
+//
+// Sequence b holds L tokens after the append, the last n of them new (n = its rows of q).  Row i
+// stands at position p = L - n + i and sees token j when
+//     j < prefix[b]   or   ( j <= p  and  (window == 0  or  p - j < window) ).
+// Its score is  s = sm_scale * q.k,  capped:  s = cap * tanh(s / cap),  then biased by distance:
+// s -= slope[head] * |p - j|.  Everything is kept in units of log2 (scores times log2 e), so that
+// a weight is one exp2.
+//
+// Rows of one KV head are packed as r = i * group + g: the group's query heads share every key
+// that is loaded, and a single new token is simply a tile with `group` rows.
+#pragma once
+
+#include "kin_attend.h"
+
+namespace kin {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct ChunkParams {
+  const uint16_t* q;              // [nnz, hq, D]
+  const uint16_t* kv;
+  const int32_t* q_indptr;        // [batch + 1]
+  const int32_t* page_indices;
+  const int32_t* page_indptr;     // [batch + 1]
+  const int32_t* last_page_len;   // [batch]
+  const float* slopes;            // [hq] or null
+  const int32_t* prefix_lens;     // [batch] or null
+  int64_t num_pages;
+  int nnz, batch, hq, hkv, group;
+  int page_size, page_shift;      // page_size == 1 << page_shift
+  int first_page_offset, window;
+  float scale_log2;               // sm_scale * log2 e
+  float cap_in, cap_log2;         // sm_scale / cap, cap * log2 e (cap_log2 == 0: no cap)
+};
+
+// One sequence of the batch as the kernels see it; positions are token indices.
+struct ChunkSeq {
+  int e0, n;        // first row of q, new tokens
+  int len;          // tokens after the append
+  int prefix;       // tokens every row sees
+  int n_pages;
+  const int32_t* pages;
+};
+
+__device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int b) {
+  ChunkSeq s;
+  s.e0 = min(max(p.q_indptr[b], 0), p.nnz);
+  s.n = min(max(p.q_indptr[b + 1], s.e0), p.nnz) - s.e0;
+  const int ps = p.page_indptr[b];
+  s.n_pages = max(p.page_indptr[b + 1] - ps, 0);
+  s.pages = p.page_indices + ps;
+  const int last = min(max(p.last_page_len[b], 0), p.page_size);
+  s.len = s.n_pages > 0 ? max((s.n_pages - 1) * p.page_size + last - p.first_page_offset, 0) : 0;
+  s.prefix = p.prefix_lens ? min(max(p.prefix_lens[b], 0), s.len) : 0;
+  return s;
+}
+
+// The token slots (tokens shifted by the first page's padding) that one row sees:
+// [first, prefix) and [lo, hi].  A row in front of the sequence (more rows than tokens) sees none.
+struct RowSpan {
+  int lo, hi, prefix;
+};
+__device__ __forceinline__ RowSpan row_span(const ChunkParams& p, const ChunkSeq& s, int i, bool valid) {
+  const int pos = s.len - s.n + i;
+  RowSpan r{0, -1, 0};
+  if (valid && pos >= 0) {
+    r.hi = pos + p.first_page_offset;
+    r.lo = (p.window > 0 ? max(pos - p.window + 1, 0) : 0) + p.first_page_offset;
+    r.prefix = s.prefix + p.first_page_offset;
+  }
+  return r;
+}
+__device__ __forceinline__ bool row_sees(const RowSpan& r, int first, int slot) {
+  return ((slot <= r.hi) & (slot >= r.lo)) | ((slot < r.prefix) & (slot >= first));
+}
+
+// tanh to about 3 units in the last place: its series up to x^9 for |x| < 1/4 (the next term is below
+// 1e-8 of the result), 1 - 2 / (exp(2x) + 1) beyond, where that no longer cancels.
+__device__ __forceinline__ float tanh_f32(float x) {
+  const float a = fabsf(x), x2 = x * x;
+  const float small = x * fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+  const float e = fast_exp2(a * (2.0f * kLog2e));
+  const float big = copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f), x);
+  return a < 0.25f ? small : big;
+}
+
+// A raw product q.k as a score in log2 units.  slope2 = slope * log2 e, dist = |p - j|.
+__device__ __forceinline__ float chunk_score(const ChunkParams& p, float raw, float slope2, int dist) {
+  const float s = p.cap_log2 != 0.f ? p.cap_log2 * tanh_f32(raw * p.cap_in) : raw * p.scale_log2;
+  return fmaf(-slope2, (float)dist, s);
+}
+
+template <bool F16>
+__device__ __forceinline__ floatx16 mfma_32x32x16(const uint4& a, const uint4& b, floatx16 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// Row of a 32x32 accumulator tile that register i of lane half h (lane / 32) holds; its column is lane % 32.
+__device__ __forceinline__ constexpr int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
+// Two fp32 to two elements in one dword, round-to-nearest-even.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const floatx2 x = {a, b};
+  if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+}
+
+// A buffer descriptor as a plain quad of scalar registers (see make_rsrc).
+__device__ __forceinline__ u32x4 rsrc_words(const void* base, int bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  return u32x4{(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, (uint32_t)bytes, 0x00020000u};
+}
+// 64 lanes x 16 bytes from the buffer straight into 1 KiB of LDS at byte offset lds_off (below 64 KiB); lanes out of the
+// buffer's range bring zeros.  Written in assembly because the compiler, which cannot tell the stages of a staging area
+// apart, puts a wait for every such load in front of the next LDS read of any stage; the kernels wait where they need to.
+// It has no register outputs.  NT: read-once data.
+template <bool NT>
+__device__ __forceinline__ void lds_load_16(u32x4 rsrc, uint32_t lds_off, int off) {
+  if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(lds_off), "v"(off), "s"(rsrc) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_off), "v"(off), "s"(rsrc) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return (uint32_t)reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p);
+}
+
+// The value of lane ^ 32.
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+// Host side: the arguments every chunk operator takes.
+int check_chunk_args(const char* fn, const void* q, const void* kv_cache, const int32_t* q_indptr, const int32_t* page_indices,
+                     const int32_t* page_indptr, const int32_t* last_page_len, int64_t nnz, int batch, int num_q_heads,
+                     int num_kv_heads, int head_dim, int page_size, int64_t num_pages, int max_pages_per_seq,
+                     int first_page_offset, float sm_scale, float softcap, int window);
+void fill_chunk_params(ChunkParams& p, const void* q, const void* kv_cache, const int32_t* q_indptr, const int32_t* page_indices,
+                       const int32_t* page_indptr, const int32_t* last_page_len, const float* slopes, const int32_t* prefix_lens,
+                       int64_t nnz, int batch, int num_q_heads, int num_kv_heads, int head_dim, int page_size, int64_t num_pages,
+                       int first_page_offset, float sm_scale, float softcap, int window);
+
+}  // namespace kin

@@ -1,0 +1,273 @@
+// Eviction from the paged cache by accumulated weight.  A sequence longer than its budget keeps, per KV
+// head, its first sink_tokens, its newest local_tokens and, of the rest, the tokens with the largest scores
+// (ties: the lowest index).  The rows that stay move up, in their order, to tokens 0 .. budget-1 of the same pages.
+//
+// Two kernels.  evict_select_kernel, a workgroup per (sequence, KV head): a radix search for the cut score,
+// then one ordered pass that writes the list of kept tokens and moves their scores.  evict_move_kernel moves the
+// K and V rows along that list, in place: a kept token never moves to a higher place, so a workgroup
+// that reads a stretch of the list before it writes it, and takes the stretches in order, overwrites only
+// rows that it has read.  K and V, and every 128 bytes of a row, move independently and get workgroups of their own.
+#include "kin_common.h"
+
+namespace kin {
+
+constexpr int kEvictThreads = 1024;
+constexpr int kEvictPer = 4;        // tokens per lane and step of the ordered pass
+constexpr int kMoveThreads = 512;
+constexpr int kMoveRows = 4;        // rows per lane in flight
+
+struct EvictParams {
+  uint16_t* kv;
+  const float* scores;     // [blocks, hkv, stride]
+  float* scores_out;       // the same layout; may be scores
+  const int32_t* page_indices;
+  const int32_t* page_indptr;
+  const int32_t* last_page_len;
+  const int32_t* slot_ids;
+  int32_t* kept;           // [batch, hkv, budget]
+  int32_t* new_lens;       // [batch]
+  int64_t num_pages;
+  int batch, hkv, page_size, page_shift, first_page_offset;
+  int num_blocks, stride, budget, sink, local;
+};
+
+// A score as an unsigned key of the same order: -0 as +0, NaN above everything.
+__device__ __forceinline__ uint32_t score_key(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+struct EvictSeq {
+  int len, n_pages, blk;
+  const int32_t* pages;
+};
+__device__ __forceinline__ EvictSeq evict_seq(const EvictParams& p, int b) {
+  EvictSeq s;
+  const int ps = p.page_indptr[b];
+  s.n_pages = max(p.page_indptr[b + 1] - ps, 0);
+  s.pages = p.page_indices + ps;
+  const int last = min(max(p.last_page_len[b], 0), p.page_size);
+  s.len = s.n_pages > 0 ? max((s.n_pages - 1) * p.page_size + last - p.first_page_offset, 0) : 0;
+  s.blk = kbar_block_of(p.slot_ids, p.num_blocks, b);
+  return s;
+}
+
+__global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams p) {
+  __shared__ uint32_t hist[256];
+  __shared__ uint32_t pick[2];   // digit that holds the cut, keys above it
+  __shared__ int2 wave_sum[kEvictThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x / p.hkv, h = blockIdx.x - b * p.hkv;
+  const EvictSeq sq = evict_seq(p, b);
+  int32_t* kept = p.kept + ((int64_t)b * p.hkv + h) * p.budget;
+  const bool known = sq.blk >= 0 && sq.len <= p.stride;
+  const int n = sq.len, m = p.budget - p.sink - p.local;
+  if (h == 0 && tid == 0) p.new_lens[b] = known ? min(n, p.budget) : n;
+  if (!known) {  // a sequence without scores keeps what it has
+    for (int i = tid; i < p.budget; i += kEvictThreads) kept[i] = -1;
+    return;
+  }
+  const int64_t at = ((int64_t)sq.blk * p.hkv + h) * p.stride;
+  const float* src = p.scores + at;
+  float* dst = p.scores_out + at;
+  if (n <= p.budget) {
+    for (int i = tid; i < p.budget; i += kEvictThreads) kept[i] = i < n ? i : -1;
+    if (src != dst)
+      for (int i = tid; i < n; i += kEvictThreads) dst[i] = src[i];
+    return;
+  }
+  // The m-th largest key of the tokens sink .. n - local - 1, eight bits at a time.
+  const int c0 = p.sink, c1 = n - p.local;
+  uint32_t cut = 0, above = 0;
+  if (m > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256) hist[tid] = 0;
+      __syncthreads();
+      for (int i = c0 + tid; i < c1; i += kEvictThreads) {
+        const uint32_t k = score_key(src[i]);
+        if (shift == 24 || (k >> (shift + 8)) == (cut >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1u);
+      }
+      __syncthreads();
+      if (wave == 0) {  // lane l sums the digits 255 - 4l .. 252 - 4l
+        uint32_t c[4], s = 0;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          c[x] = hist[255 - 4 * lane - x];
+          s += c[x];
+        }
+        uint32_t before = wave_inclusive_sum(s) - s + above;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if (before < (uint32_t)m && before + c[x] >= (uint32_t)m) {
+            pick[0] = 255 - 4 * lane - x;
+            pick[1] = before;
+          }
+          before += c[x];
+        }
+      }
+      __syncthreads();
+      cut |= pick[0] << shift;
+      above = pick[1];
+      __syncthreads();
+    }
+  }
+  const int ties = m - (int)above;  // tokens with the cut score itself that stay, from the lowest index on
+  // Ordered pass: a wave owns 64 * kEvictPer tokens of a step; place = tokens kept for good before + ties kept before.
+  int sure0 = 0, tie0 = 0;
+  for (int base = 0; base < n; base += kEvictThreads * kEvictPer) {
+    float x[kEvictPer];
+    uint64_t sure[kEvictPer], tie[kEvictPer];
+    int ns = 0, nt = 0;
+    const int first = base + wave * 64 * kEvictPer + lane;
+#pragma unroll
+    for (int j = 0; j < kEvictPer; ++j) {
+      const int i = first + j * 64;
+      x[j] = i < n ? src[i] : 0.f;
+      const uint32_t k = score_key(x[j]);
+      const bool mid = i >= c0 && i < c1;
+      sure[j] = __ballot(i < n && (!mid || (m > 0 && k > cut)));
+      tie[j] = __ballot(mid && m > 0 && k == cut);
+      ns += __popcll(sure[j]);
+      nt += __popcll(tie[j]);
+    }
+    if (lane == 0) wave_sum[wave] = make_int2(ns, nt);
+    __syncthreads();
+    int s = sure0, t = tie0;
+    for (int w = 0; w < kEvictThreads / 64; ++w) {
+      const int2 v = wave_sum[w];
+      if (w < wave) {
+        s += v.x;
+        t += v.y;
+      }
+      sure0 += v.x;
+      tie0 += v.y;
+    }
+    __syncthreads();  // also: every score of this step is read before any place below it is written
+    const uint64_t lower = (1ull << lane) - 1;
+#pragma unroll
+    for (int j = 0; j < kEvictPer; ++j) {
+      const int i = first + j * 64;
+      const int sb = s + __popcll(sure[j] & lower), tb = t + __popcll(tie[j] & lower);
+      const bool keep = ((sure[j] >> lane) & 1) || (((tie[j] >> lane) & 1) && tb < ties);
+      if (keep) {
+        const int place = sb + min(tb, ties);
+        kept[place] = i;
+        dst[place] = x[j];
+      }
+      s += __popcll(sure[j]);
+      t += __popcll(tie[j]);
+    }
+  }
+  __syncthreads();
+  for (int i = p.budget + tid; i < n; i += kEvictThreads) dst[i] = 0.f;
+}
+
+// blockIdx.x: 128-byte part of the row, K or V, head, sequence (part fastest).
+__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p, int parts, int row_bytes) {
+  const int tid = threadIdx.x;
+  int x = blockIdx.x;
+  const int part = x % parts;
+  x /= parts;
+  const int plane = x & 1;
+  x >>= 1;
+  const int h = x % p.hkv, b = x / p.hkv;
+  const EvictSeq sq = evict_seq(p, b);
+  if (sq.blk < 0 || sq.len > p.stride || sq.len <= p.budget) return;
+  const int32_t* kept = p.kept + ((int64_t)b * p.hkv + h) * p.budget;
+  const int64_t page_bytes = 2ll * p.page_size * row_bytes;
+  char* base = reinterpret_cast<char*>(p.kv) + (int64_t)plane * p.page_size * row_bytes + (int64_t)h * (row_bytes / p.hkv) +
+               part * 128 + (tid & 7) * 16;
+  auto row_of = [&](int token) -> char* {
+    const int at = token + p.first_page_offset;
+    const int id = sq.pages[at >> p.page_shift];
+    if (id < 0 || (int64_t)id >= p.num_pages) return nullptr;
+    return base + (int64_t)id * page_bytes + (int64_t)(at & (p.page_size - 1)) * row_bytes;
+  };
+  constexpr int kStep = kMoveThreads / 8;
+  for (int first = p.sink; first < p.budget; first += kStep * kMoveRows) {
+    u32x4 v[kMoveRows];
+    char* to[kMoveRows];
+#pragma unroll
+    for (int j = 0; j < kMoveRows; ++j) {
+      const int dst = first + j * kStep + (tid >> 3);
+      const int src = dst < p.budget ? kept[dst] : dst;
+      to[j] = nullptr;
+      if (src != dst) {  // tokens in front of the first gap stay where they are
+        const char* from = row_of(src);
+        to[j] = from ? row_of(dst) : nullptr;
+        if (to[j]) v[j] = *reinterpret_cast<const u32x4*>(from);
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0);  // every row of the stretch is in registers ...
+    __syncthreads();                // ... in all waves, before any of them is overwritten
+#pragma unroll
+    for (int j = 0; j < kMoveRows; ++j)
+      if (to[j]) *reinterpret_cast<u32x4*>(to[j]) = v[j];
+  }
+}
+
+static int evict_tokens_impl(const char* fn, void* kv_cache, const float* scores, float* scores_out, const int32_t* page_indices,
+                             const int32_t* page_indptr, const int32_t* last_page_len, int32_t* kept, int32_t* new_lens,
+                             int batch, int num_kv_heads, int head_dim, int page_size, int64_t num_pages, int first_page_offset,
+                             int budget, int sink_tokens, int local_tokens, int score_blocks, int score_stride,
+                             const int32_t* slot_ids, kin_stream_t stream) {
+  if (!kv_cache || !scores || !scores_out || !page_indices || !page_indptr || !last_page_len || !kept || !new_lens)
+    return fail(KIN_ERR_NULL_POINTER, "%s: null pointer argument", fn);
+  if (int st = check_common_dims(fn, batch, num_kv_heads, num_kv_heads, head_dim, page_size, true)) return st;
+  if (int st = check_first_page_offset(fn, first_page_offset, page_size)) return st;
+  if (num_pages < 1) return fail(KIN_ERR_BAD_SHAPE, "%s: num_pages=%lld must be >= 1", fn, (long long)num_pages);
+  if (sink_tokens < 0 || local_tokens < 0 || budget < 1 || (int64_t)sink_tokens + local_tokens > budget)
+    return fail(KIN_ERR_BAD_SHAPE, "%s: budget=%d must be positive and hold sink_tokens=%d and local_tokens=%d", fn, budget,
+                sink_tokens, local_tokens);
+  if (score_stride < 1 || score_blocks < 0 || (!slot_ids && score_blocks < batch) || (slot_ids && score_blocks < 1))
+    return fail(KIN_ERR_BAD_SHAPE, "%s: scores of %d rows of %d entries for batch=%d", fn, score_blocks, score_stride, batch);
+  if (!aligned16(kv_cache)) return fail(KIN_ERR_MISALIGNED, "%s: kv_cache must be 16-byte aligned", fn);
+  const int parts = head_dim * 2 / 128;
+  if ((int64_t)batch * num_kv_heads * 2 * parts > 0x7fffffffLL)
+    return fail(KIN_ERR_UNSUPPORTED, "%s: batch*num_kv_heads is too large", fn);
+  if (batch == 0) return KIN_OK;
+  EvictParams p;
+  p.kv = static_cast<uint16_t*>(kv_cache);
+  p.scores = scores;
+  p.scores_out = scores_out;
+  p.page_indices = page_indices;
+  p.page_indptr = page_indptr;
+  p.last_page_len = last_page_len;
+  p.slot_ids = slot_ids;
+  p.kept = kept;
+  p.new_lens = new_lens;
+  p.num_pages = num_pages;
+  p.batch = batch;
+  p.hkv = num_kv_heads;
+  p.page_size = page_size;
+  p.page_shift = 4 + page_tile_shift(page_size);
+  p.first_page_offset = first_page_offset;
+  p.num_blocks = score_blocks;
+  p.stride = score_stride;
+  p.budget = budget;
+  p.sink = sink_tokens;
+  p.local = local_tokens;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  evict_select_kernel<<<(unsigned)(batch * num_kv_heads), kEvictThreads, 0, s>>>(p);
+  if (int st = check_hip(hipGetLastError(), "evict_select_kernel launch")) return st;
+  evict_move_kernel<<<(unsigned)(batch * num_kv_heads * 2 * parts), kMoveThreads, 0, s>>>(p, parts, num_kv_heads * head_dim * 2);
+  return check_hip(hipGetLastError(), "evict_move_kernel launch");
+}
+
+}  // namespace kin
+
+extern "C" {
+
+/* Rows are moved as bytes: bfloat16 and float16 caches alike. */
+int kin_evict_tokens(void* kv_cache, const float* scores, float* scores_out, const int32_t* page_indices,
+                     const int32_t* page_indptr, const int32_t* last_page_len, int32_t* kept, int32_t* new_lens, int batch,
+                     int num_kv_heads, int head_dim, int page_size, int64_t num_pages, int first_page_offset, int budget,
+                     int sink_tokens, int local_tokens, int score_blocks, int score_stride, const int32_t* slot_ids,
+                     kin_stream_t stream) {
+  return kin::evict_tokens_impl("kin_evict_tokens", kv_cache, scores, scores_out, page_indices, page_indptr, last_page_len, kept,
+                                new_lens, batch, num_kv_heads, head_dim, page_size, num_pages, first_page_offset, budget,
+                                sink_tokens, local_tokens, score_blocks, score_stride, slot_ids, stream);
+}
+
+}  // extern "C"

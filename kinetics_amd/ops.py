@@ -12,6 +12,7 @@ traceable by ``torch.compile(fullgraph=True)``.
 from __future__ import annotations
 
 import contextlib
+import math
 from ctypes import c_void_p
 from typing import Optional
 
@@ -749,6 +750,176 @@ def check_page_table(page_indices, page_indptr, last_page_len, page_size, num_pa
 
 
 # ---------------------------------------------------------------------------
+# Chunks of new tokens: attention, the weight it gave, eviction by weight
+# ---------------------------------------------------------------------------
+
+
+def chunk_workspace_bytes(nnz: int, batch: int, num_q_heads: int, num_kv_heads: int, max_pages_per_seq: int,
+                          page_size: int = PAGE_SIZE, head_dim: int = HEAD_DIM, num_splits: int = 0) -> int:
+    """Bytes of workspace ``paged_chunk_attention`` needs for this shape (0: none)."""
+    return int(_lib.load().kin_chunk_workspace_bytes(int(nnz), int(batch), int(num_q_heads), int(num_kv_heads),
+                                                     int(max_pages_per_seq), int(page_size), int(head_dim), int(num_splits)))
+
+
+def _chunk_args(q, kv_cache, q_indptr, page_indices, page_indptr, last_page_len, slopes, prefix_lens):
+    num_pages, page_size, num_kv_heads, head_dim = _cache_dims(kv_cache)
+    dev = kv_cache.device
+    _require(q, "q", kv_cache.dtype, 3, dev)
+    nnz, num_q_heads, qd = q.shape
+    if qd != head_dim:
+        raise ValueError(f"q head_dim {qd} != kv_cache head_dim {head_dim}")
+    _require(q_indptr, "q_indptr", torch.int32, 1, dev)
+    batch = q_indptr.numel() - 1
+    if batch < 0:
+        raise ValueError("q_indptr must have batch+1 entries")
+    if last_page_len is None:
+        raise TypeError("last_page_len is required")
+    _table(page_indices, page_indptr, last_page_len, batch, dev)
+    if slopes is not None:
+        _require(slopes, "slopes", torch.float32, 1, dev)
+        if slopes.numel() != num_q_heads:
+            raise ValueError(f"slopes must have num_q_heads={num_q_heads} entries, got {slopes.numel()}")
+    if prefix_lens is not None:
+        _require(prefix_lens, "prefix_lens", torch.int32, 1, dev)
+        if prefix_lens.numel() != batch:
+            raise ValueError(f"prefix_lens must have batch={batch} entries, got {prefix_lens.numel()}")
+    return dev, nnz, batch, num_q_heads, num_kv_heads, head_dim, page_size, num_pages
+
+
+def paged_chunk_attention(q, kv_cache, q_indptr, page_indices, page_indptr, last_page_len, max_pages_per_seq, out=None, lse=None,
+                          workspace=None, sm_scale: float = 0.0, softcap: float = 0.0, window: int = 0, slopes=None,
+                          prefix_lens=None, first_page_offset: int = 0, num_splits: int = 0):
+    """Attention of a ragged batch of new tokens over the paged cache: sequence b brings the rows
+    ``q_indptr[b] .. q_indptr[b+1]-1`` of ``q`` [nnz, num_q_heads, head_dim] -- one token, a few, a whole prompt, or
+    none -- whose keys and values are already in the cache (the page table describes it after the append).  Causal;
+    with ``window`` over the newest ``window`` tokens only; the first ``prefix_lens[b]`` tokens (int32 [batch]) are
+    seen by every row.  ``softcap``: scores become ``softcap * tanh(score / softcap)``; ``slopes`` (fp32 [num_q_heads]):
+    minus ``slope * distance``.  Covers LiteSys' prefill (LiteSys/litesys/attention/batch_cache.py:112-145), many
+    requests at a time.  ``lse`` (fp32 [nnz, num_q_heads]) receives the log-sum-exp.  ``workspace`` (uint8,
+    ``chunk_workspace_bytes``; allocated here when None and needed).  Rows that belong to no sequence are left as
+    they were in ``out`` and ``lse`` (unset in an ``out`` allocated here).  Returns ``out`` [nnz, num_q_heads, head_dim]."""
+    dev, nnz, batch, hq, hkv, d, ps, num_pages = _chunk_args(q, kv_cache, q_indptr, page_indices, page_indptr, last_page_len,
+                                                             slopes, prefix_lens)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _require(out, "out", kv_cache.dtype, 3, dev)
+        if out.shape != q.shape:
+            raise ValueError(f"out shape {tuple(out.shape)} != q shape {tuple(q.shape)}")
+    if lse is not None:
+        _require(lse, "lse", torch.float32, 2, dev)
+        if tuple(lse.shape) != (nnz, hq):
+            raise ValueError(f"lse must be [{nnz}, {hq}], got {tuple(lse.shape)}")
+    if workspace is not None:
+        _require(workspace, "workspace", torch.uint8, 1, dev)
+    else:
+        need = chunk_workspace_bytes(nnz, batch, hq, hkv, max_pages_per_seq, ps, d, num_splits)
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(
+            _entry(lib, "kin_paged_chunk_attention", kv_cache.dtype)(
+                _ptr(q), _ptr(kv_cache), _ptr(q_indptr), _ptr(page_indices), _ptr(page_indptr), _ptr(last_page_len), _ptr(slopes),
+                _ptr(prefix_lens), _ptr(out), _ptr(lse), _ptr(workspace), 0 if workspace is None else workspace.numel(), nnz,
+                batch, hq, hkv, d, ps, num_pages, int(max_pages_per_seq), int(first_page_offset), float(sm_scale),
+                float(softcap), int(window), int(num_splits), _stream(dev),
+            )
+        )
+    return out
+
+
+def _score_rows(scores, name, batch, num_kv_heads, dev, slot_ids):
+    """(blocks, stride) of a score tensor [blocks, num_kv_heads, stride] and the pointer of ``slot_ids``."""
+    _require(scores, name, torch.float32, 3, dev)
+    if scores.shape[1] != num_kv_heads or (slot_ids is None and scores.shape[0] < batch):
+        raise ValueError(f"{name} must be [batch={batch}, {num_kv_heads}, tokens] ([slots, ...] with slot_ids), "
+                         f"got {tuple(scores.shape)}")
+    if slot_ids is not None:
+        _require(slot_ids, "slot_ids", torch.int32, 1, dev)
+        if slot_ids.numel() != batch:
+            raise ValueError(f"slot_ids must have batch={batch} entries, got {slot_ids.numel()}")
+    return scores.shape[0], scores.shape[2]
+
+
+def attention_mass(q, kv_cache, lse, scores, q_indptr, page_indices, page_indptr, last_page_len, max_pages_per_seq,
+                   sm_scale: float = 0.0, softcap: float = 0.0, window: int = 0, slopes=None, prefix_lens=None,
+                   first_page_offset: int = 0, slot_ids=None) -> None:
+    """Add to ``scores`` (fp32 [batch, num_kv_heads, tokens]) the attention weight that every cached token received from
+    the rows of ``q``, summed over the rows and the group's query heads: ``exp(score - lse)`` with the ``lse`` that
+    ``paged_chunk_attention`` (or a decode call) wrote for the same arguments.  In place and in a fixed order of
+    additions.  ``slot_ids`` (int32 [batch], optional): ``scores`` is laid out by cache slot."""
+    dev, nnz, batch, hq, hkv, d, ps, num_pages = _chunk_args(q, kv_cache, q_indptr, page_indices, page_indptr, last_page_len,
+                                                             slopes, prefix_lens)
+    _require(lse, "lse", torch.float32, 2, dev)
+    if tuple(lse.shape) != (nnz, hq):
+        raise ValueError(f"lse must be [{nnz}, {hq}], got {tuple(lse.shape)}")
+    blocks, stride = _score_rows(scores, "scores", batch, hkv, dev, slot_ids)
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(
+            _entry(lib, "kin_attention_mass", kv_cache.dtype)(
+                _ptr(q), _ptr(kv_cache), _ptr(lse), _ptr(scores), _ptr(q_indptr), _ptr(page_indices), _ptr(page_indptr),
+                _ptr(last_page_len), _ptr(slopes), _ptr(prefix_lens), nnz, batch, hq, hkv, d, ps, num_pages,
+                int(max_pages_per_seq), int(first_page_offset), float(sm_scale), float(softcap), int(window), blocks, stride,
+                _ptr(slot_ids), _stream(dev),
+            )
+        )
+
+
+def evict_tokens(kv_cache, scores, page_indices, page_indptr, last_page_len, budget: int, sink_tokens: int = 4,
+                 local_tokens: int = 32, first_page_offset: int = 0, scores_out=None, kept=None, new_lens=None, slot_ids=None):
+    """Cut every sequence that holds more than ``budget`` tokens down to it: per KV head the first ``sink_tokens``, the
+    newest ``local_tokens`` and the tokens with the largest ``scores`` in between stay (ties: the lowest index; NaN counts
+    as largest) and move up, in their order, inside the sequence's own pages, which no other sequence may share.
+    ``scores`` (fp32 [batch, num_kv_heads, tokens], as ``attention_mass`` accumulates them) moves along, in place or
+    into ``scores_out``; freed entries become 0.  Returns ``(kept, new_lens)``: int32 [batch, num_kv_heads, budget], the
+    tokens that stayed, padded with -1, and int32 [batch], the new lengths, from which the caller builds the new page
+    table (and, if it keeps mean keys, ``build_kbar``)."""
+    num_pages, page_size, hkv, d = _cache_dims(kv_cache)
+    dev = kv_cache.device
+    _require(page_indptr, "page_indptr", torch.int32, 1, dev)
+    batch = page_indptr.numel() - 1
+    if batch < 0:
+        raise ValueError("page_indptr must have batch+1 entries")
+    if last_page_len is None:
+        raise TypeError("last_page_len is required")
+    _table(page_indices, page_indptr, last_page_len, batch, dev)
+    blocks, stride = _score_rows(scores, "scores", batch, hkv, dev, slot_ids)
+    if scores_out is None:
+        scores_out = scores
+    else:
+        _require(scores_out, "scores_out", torch.float32, 3, dev)
+        if scores_out.shape != scores.shape:
+            raise ValueError(f"scores_out shape {tuple(scores_out.shape)} != scores shape {tuple(scores.shape)}")
+        gap = scores_out.data_ptr() - scores.data_ptr()
+        if gap and abs(gap) < scores.numel() * 4:
+            raise ValueError("scores_out must be scores itself or not overlap it")
+    if kept is None:
+        kept = torch.empty(batch, hkv, max(int(budget), 0), dtype=torch.int32, device=dev)
+    else:
+        _require(kept, "kept", torch.int32, 3, dev)
+        if tuple(kept.shape) != (batch, hkv, budget):
+            raise ValueError(f"kept must be [{batch}, {hkv}, {budget}], got {tuple(kept.shape)}")
+    if new_lens is None:
+        new_lens = torch.empty(batch, dtype=torch.int32, device=dev)
+    else:
+        _require(new_lens, "new_lens", torch.int32, 1, dev)
+        if new_lens.numel() != batch:
+            raise ValueError(f"new_lens must have batch={batch} entries, got {new_lens.numel()}")
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(
+            lib.kin_evict_tokens(
+                _ptr(kv_cache), _ptr(scores), _ptr(scores_out), _ptr(page_indices), _ptr(page_indptr), _ptr(last_page_len),
+                _ptr(kept), _ptr(new_lens), batch, hkv, d, page_size, num_pages, int(first_page_offset), int(budget),
+                int(sink_tokens), int(local_tokens), blocks, stride, _ptr(slot_ids), _stream(dev),
+            )
+        )
+    return kept, new_lens
+
+
+# ---------------------------------------------------------------------------
 # Row-wise layer kernels around the attention path
 # ---------------------------------------------------------------------------
 
@@ -831,6 +1002,81 @@ def qkv_norm_split(qkv, q_weight, k_weight, eps: float, num_q_heads: int, num_kv
         _lib.check(_entry(lib, "kin_qkv_norm_split", dt)(_ptr(qkv), stride, _ptr(q_weight), _ptr(k_weight), float(eps),
                                                          _ptr(q), _ptr(k), _ptr(v), batch, int(num_q_heads),
                                                          int(num_kv_heads), head_dim, _stream(dev)))
+    return q, k, v
+
+
+def rope_table(head_dim: int, theta: float = 1000000.0, sections=None, interleaved: bool = False, inv_freq=None, device="cuda"):
+    """``(freq, axis)`` for ``qkv_norm_rope_split``, built once per model: int64 [head_dim/2], turns per position as a
+    fraction of 2^64, and int32 [head_dim/2], the axis whose position turns each pair.  ``theta``: base of the usual
+    frequencies ``theta ** (-2i / head_dim)`` (LiteSys/litesys/models/qwen3.py:49-61), or give ``inv_freq``
+    (head_dim/2 radians per position, e.g. scaled ones).  ``sections``: how many pairs each axis turns, in the order of the
+    rows of ``positions`` (default: one axis, all of them); contiguous, or with ``interleaved`` dealt out in turn as
+    long as an axis has pairs left.  Pairs beyond the sections' sum are not turned."""
+    pairs = int(head_dim) // 2
+    if inv_freq is None:
+        inv = [float(theta) ** (-2.0 * i / head_dim) for i in range(pairs)]
+    else:
+        inv = [float(x) for x in inv_freq]
+        if len(inv) != pairs:
+            raise ValueError(f"inv_freq must have head_dim/2={pairs} entries, got {len(inv)}")
+    if not all(math.isfinite(x) for x in inv):
+        raise ValueError("frequencies must be finite")
+    left = [pairs] if sections is None else [int(n) for n in sections]
+    if not left or min(left) < 0 or sum(left) > pairs:
+        raise ValueError(f"sections must be non-negative and sum to at most head_dim/2={pairs}, got {left}")
+    axis = []
+    if interleaved:
+        while any(left):
+            for a, n in enumerate(left):
+                if n:
+                    left[a] -= 1
+                    axis.append(a)
+    else:
+        axis = [a for a, n in enumerate(left) for _ in range(n)]
+    axis += [-1] * (pairs - len(axis))
+    freq = []
+    for x in inv:
+        turns = int(round(x / (2.0 * math.pi) * 2.0 ** 64)) % 2 ** 64
+        freq.append(turns - 2 ** 64 if turns >= 2 ** 63 else turns)
+    return (torch.tensor(freq, dtype=torch.int64, device=device), torch.tensor(axis, dtype=torch.int32, device=device))
+
+
+def qkv_norm_rope_split(qkv, q_weight, k_weight, eps: float, positions, freq, axis, num_q_heads: int, num_kv_heads: int):
+    """``qkv_norm_split`` with rotary positions: contiguous ``q[tokens, Hq, D]``, ``k[tokens, Hkv, D]``,
+    ``v[tokens, Hkv, D]`` from the fused projection, the q and k heads RMS-normalised (weights None: not) and their
+    pairs (i, i + D/2) turned by ``positions[axis[i]] * frequency[i]``
+    (the rotation of LiteSys/litesys/models/model_utils.py:17-52).  ``positions``: int32 [axes, tokens], or [tokens] for one axis;
+    ``freq``, ``axis``: ``rope_table``.  Angles are exact for every int32 position; one rounding at the end."""
+    tokens, width, stride = _row_view(qkv, "qkv")
+    dev, dt = qkv.device, qkv.dtype
+    _require(freq, "freq", torch.int64, 1, dev)
+    _require(axis, "axis", torch.int32, 1, dev)
+    _require(positions, "positions", torch.int32, (1, 2), dev)
+    head_dim = 2 * freq.numel()
+    if head_dim not in HEAD_DIMS or axis.numel() != freq.numel():
+        raise ValueError(f"freq and axis must have head_dim/2 entries each, head_dim one of {HEAD_DIMS}; "
+                         f"got {freq.numel()} and {axis.numel()}")
+    axes = 1 if positions.dim() == 1 else positions.shape[0]
+    if positions.shape[-1] != tokens or axes < 1:
+        raise ValueError(f"positions must be [axes, {tokens}] or [{tokens}], got {tuple(positions.shape)}")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("q_weight and k_weight must both be given or both be None")
+    if q_weight is not None:
+        _require(q_weight, "q_weight", dt, 1, dev)
+        _require(k_weight, "k_weight", dt, 1, dev)
+        if q_weight.numel() != head_dim or k_weight.numel() != head_dim:
+            raise ValueError(f"q_weight and k_weight must have head_dim={head_dim} entries, got {q_weight.numel()} and {k_weight.numel()}")
+    if width != (num_q_heads + 2 * num_kv_heads) * head_dim:
+        raise ValueError(f"qkv rows have {width} elements, expected (Hq + 2*Hkv) * {head_dim} = "
+                         f"{(num_q_heads + 2 * num_kv_heads) * head_dim}")
+    q = torch.empty(tokens, num_q_heads, head_dim, dtype=dt, device=dev)
+    k = torch.empty(tokens, num_kv_heads, head_dim, dtype=dt, device=dev)
+    v = torch.empty(tokens, num_kv_heads, head_dim, dtype=dt, device=dev)
+    lib = _lib.load()
+    with _on(dev):
+        _lib.check(_entry(lib, "kin_qkv_norm_rope_split", dt)(
+            _ptr(qkv), stride, _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(positions), axes, _ptr(freq), _ptr(axis), _ptr(q),
+            _ptr(k), _ptr(v), tokens, int(num_q_heads), int(num_kv_heads), head_dim, _stream(dev)))
     return q, k, v
 
 
@@ -1061,3 +1307,83 @@ def _gated_act_impl(gate, up, act):
 @torch.library.register_fake("kinetics::gated_act")
 def _gated_act_fake(gate, up, act):
     return torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+
+
+# Chunks of new tokens, and the rotary form of the split.
+torch.library.define(
+    "kinetics::paged_chunk_attention",
+    "(Tensor q, Tensor kv_cache, Tensor q_indptr, Tensor page_indices, Tensor page_indptr, Tensor last_page_len, "
+    "int max_pages_per_seq, Tensor(a!)? lse=None, Tensor(b!)? workspace=None, float sm_scale=0.0, float softcap=0.0, "
+    "int window=0, Tensor? slopes=None, Tensor? prefix_lens=None, int first_page_offset=0, int num_splits=0) -> Tensor",
+)
+torch.library.define(
+    "kinetics::attention_mass",
+    "(Tensor q, Tensor kv_cache, Tensor lse, Tensor(a!) scores, Tensor q_indptr, Tensor page_indices, Tensor page_indptr, "
+    "Tensor last_page_len, int max_pages_per_seq, float sm_scale=0.0, float softcap=0.0, int window=0, Tensor? slopes=None, "
+    "Tensor? prefix_lens=None, int first_page_offset=0, Tensor? slot_ids=None) -> ()",
+)
+torch.library.define(
+    "kinetics::evict_tokens",
+    "(Tensor(a!) kv_cache, Tensor(b!) scores, Tensor page_indices, Tensor page_indptr, Tensor last_page_len, int budget, "
+    "int sink_tokens=4, int local_tokens=32, int first_page_offset=0, Tensor? slot_ids=None) -> (Tensor, Tensor)",
+)
+torch.library.define(
+    "kinetics::qkv_norm_rope_split",
+    "(Tensor qkv, Tensor? q_weight, Tensor? k_weight, float eps, Tensor positions, Tensor freq, Tensor axis, int num_q_heads, "
+    "int num_kv_heads) -> (Tensor, Tensor, Tensor)",
+)
+
+
+@torch.library.impl("kinetics::paged_chunk_attention", "cuda")
+def _chunk_impl(q, kv_cache, q_indptr, page_indices, page_indptr, last_page_len, max_pages_per_seq, lse=None, workspace=None,
+                sm_scale=0.0, softcap=0.0, window=0, slopes=None, prefix_lens=None, first_page_offset=0, num_splits=0):
+    return paged_chunk_attention(q, kv_cache, q_indptr, page_indices, page_indptr, last_page_len, max_pages_per_seq, lse=lse,
+                                 workspace=workspace, sm_scale=sm_scale, softcap=softcap, window=window, slopes=slopes,
+                                 prefix_lens=prefix_lens, first_page_offset=first_page_offset, num_splits=num_splits)
+
+
+@torch.library.register_fake("kinetics::paged_chunk_attention")
+def _chunk_fake(q, kv_cache, q_indptr, page_indices, page_indptr, last_page_len, max_pages_per_seq, lse=None, workspace=None,
+                sm_scale=0.0, softcap=0.0, window=0, slopes=None, prefix_lens=None, first_page_offset=0, num_splits=0):
+    return torch.empty_like(q)
+
+
+@torch.library.impl("kinetics::attention_mass", "cuda")
+def _mass_impl(q, kv_cache, lse, scores, q_indptr, page_indices, page_indptr, last_page_len, max_pages_per_seq, sm_scale=0.0,
+               softcap=0.0, window=0, slopes=None, prefix_lens=None, first_page_offset=0, slot_ids=None):
+    attention_mass(q, kv_cache, lse, scores, q_indptr, page_indices, page_indptr, last_page_len, max_pages_per_seq,
+                   sm_scale=sm_scale, softcap=softcap, window=window, slopes=slopes, prefix_lens=prefix_lens,
+                   first_page_offset=first_page_offset, slot_ids=slot_ids)
+
+
+@torch.library.register_fake("kinetics::attention_mass")
+def _mass_fake(q, kv_cache, lse, scores, q_indptr, page_indices, page_indptr, last_page_len, max_pages_per_seq, sm_scale=0.0,
+               softcap=0.0, window=0, slopes=None, prefix_lens=None, first_page_offset=0, slot_ids=None):
+    return None
+
+
+@torch.library.impl("kinetics::evict_tokens", "cuda")
+def _evict_impl(kv_cache, scores, page_indices, page_indptr, last_page_len, budget, sink_tokens=4, local_tokens=32,
+                first_page_offset=0, slot_ids=None):
+    return evict_tokens(kv_cache, scores, page_indices, page_indptr, last_page_len, budget, sink_tokens=sink_tokens,
+                        local_tokens=local_tokens, first_page_offset=first_page_offset, slot_ids=slot_ids)
+
+
+@torch.library.register_fake("kinetics::evict_tokens")
+def _evict_fake(kv_cache, scores, page_indices, page_indptr, last_page_len, budget, sink_tokens=4, local_tokens=32,
+                first_page_offset=0, slot_ids=None):
+    batch = page_indptr.numel() - 1
+    return (page_indptr.new_empty(batch, kv_cache.shape[3], budget), page_indptr.new_empty(batch))
+
+
+@torch.library.impl("kinetics::qkv_norm_rope_split", "cuda")
+def _rope_impl(qkv, q_weight, k_weight, eps, positions, freq, axis, num_q_heads, num_kv_heads):
+    return qkv_norm_rope_split(qkv, q_weight, k_weight, eps, positions, freq, axis, num_q_heads, num_kv_heads)
+
+
+@torch.library.register_fake("kinetics::qkv_norm_rope_split")
+def _rope_fake(qkv, q_weight, k_weight, eps, positions, freq, axis, num_q_heads, num_kv_heads):
+    tokens = qkv.numel() // qkv.shape[-1]
+    head_dim = 2 * freq.numel()
+    return (qkv.new_empty(tokens, num_q_heads, head_dim), qkv.new_empty(tokens, num_kv_heads, head_dim),
+            qkv.new_empty(tokens, num_kv_heads, head_dim))
