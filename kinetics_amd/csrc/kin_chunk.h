@@ -81,20 +81,51 @@ __device__ __forceinline__ bool row_sees(const RowSpan& r, int first, int slot) 
   return ((slot <= r.hi) & (slot >= r.lo)) | ((slot < r.prefix) & (slot >= first));
 }
 
-// tanh to about 3 units in the last place: its series up to x^9 for |x| < 1/4 (the next term is below
-// 1e-8 of the result), 1 - 2 / (exp(2x) + 1) beyond, where that no longer cancels.
-__device__ __forceinline__ float tanh_f32(float x) {
-  const float a = fabsf(x), x2 = x * x;
-  const float small = x * fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-  const float e = fast_exp2(a * (2.0f * kLog2e));
-  const float big = copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f), x);
-  return a < 0.25f ? small : big;
+// tanh to about 3 units in the last place.  Below 3/4 x P(x^2) with P of degree 5 (least largest relative error on
+// that range, 3e-8 by its coefficients, 1.6e-7 with the fp32 roundings); beyond, 1 - 2 / (exp(2x) + 1), which no longer cancels.
+constexpr float kTanhSmall = 0.75f;
+__device__ __forceinline__ float tanh_small(float x) {
+  const float t = x * x;
+  float y = fmaf(t, -0.004716257564723492f, 0.01958290860056877f);
+  y = fmaf(t, y, -0.05334443226456642f);
+  y = fmaf(t, y, 0.1332540661096573f);
+  y = fmaf(t, y, -0.33332958817481995f);
+  return x * fmaf(t, y, 1.0f);
+}
+__device__ __forceinline__ float tanh_large(float x) {
+  const float e = fast_exp2(fabsf(x) * (2.0f * kLog2e));
+  return copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f), x);
 }
 
-// A raw product q.k as a score in log2 units.  slope2 = slope * log2 e, dist = |p - j|.
-__device__ __forceinline__ float chunk_score(const ChunkParams& p, float raw, float slope2, int dist) {
-  const float s = p.cap_log2 != 0.f ? p.cap_log2 * tanh_f32(raw * p.cap_in) : raw * p.scale_log2;
-  return fmaf(-slope2, (float)dist, s);
+// 16 raw products q.k of a lane as scores in log2 units, capped (without the distance bias).  Scores far below the
+// cap, which is what a cap is for, take the short form: 8 instead of about 24 issue slots each, chosen per block.
+__device__ __forceinline__ void cap_scores(const ChunkParams& p, floatx16& s) {
+  if (p.cap_log2 == 0.f) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] *= p.scale_log2;
+    return;
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(s[e]));
+  if (!__ballot(!(top * p.cap_in < kTanhSmall))) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = p.cap_log2 * tanh_small(s[e] * p.cap_in);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float x = s[e] * p.cap_in;
+      s[e] = p.cap_log2 * (fabsf(x) < kTanhSmall ? tanh_small(x) : tanh_large(x));
+    }
+  }
+}
+
+// Row r of a staged tile of head rows holds its 16-byte chunk c at position c ^ row_swizzle(r): 16 rows read at one chunk
+// column and 4 rows read at 4 neighbouring ones both cover all LDS banks once.
+template <int HD>
+__device__ __forceinline__ constexpr int row_swizzle(int row) {
+  if (HD == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+  return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
 template <bool F16>

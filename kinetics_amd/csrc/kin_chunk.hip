@@ -17,9 +17,6 @@
 // four keys of one column.  P never leaves the registers.  P is rounded to the cache's element type
 // for the matrix unit (half a unit in the last place, as the result itself); the running sum and
 // maximum, and O, are fp32.
-//
-// Row r of a staged tile holds its 16-byte chunk c at position c ^ kv_swizzle(r): 16 rows read at one
-// chunk column (K) and 4 rows read at 4 neighbouring ones (V) both cover all banks once.
 #include "kin_chunk.h"
 
 namespace kin {
@@ -39,12 +36,6 @@ struct ChunkAttnParams {
 };
 
 typedef short shortx4 __attribute__((ext_vector_type(4)));
-
-template <int HD>
-__device__ __forceinline__ constexpr int kv_swizzle(int row) {
-  if (HD == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
-  return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
-}
 
 // First row tile of sequence b: tiles are numbered so that every sequence has room for its rows
 // whatever the others bring, without a scan: floor(q_indptr[b] * group / 128) + b.
@@ -134,17 +125,21 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
     for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < HD / 16; ++kk) {
-      const uint4 a = *reinterpret_cast<const uint4*>(k + (t * 32 + col) * kRowB + (((2 * kk + half) ^ kv_swizzle<HD>(col)) * 16));
+      const uint4 a = *reinterpret_cast<const uint4*>(k + (t * 32 + col) * kRowB + (((2 * kk + half) ^ row_swizzle<HD>(col)) * 16));
       s[t] = mfma_32x32x16<F16>(a, w.q[kk], s[t]);
     }
   }
   after_k();
   if constexpr (EXTRA) {
-    const int pos = w.span.hi;  // the row's own token slot
 #pragma unroll
-    for (int t = 0; t < NSUB; ++t)
+    for (int t = 0; t < NSUB; ++t) cap_scores(p, s[t]);
+    if (p.slopes) {
+      const int pos = w.span.hi;  // the row's own token slot
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[t][e] = chunk_score(p, s[t][e], w.slope2, abs(pos - (slot0 + t * 32 + acc_row(e, half))));
+      for (int t = 0; t < NSUB; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[t][e] = fmaf(-w.slope2, (float)abs(pos - (slot0 + t * 32 + acc_row(e, half))), s[t][e]);
+    }
   }
   if (masked) {
 #pragma unroll
@@ -198,7 +193,7 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int row = 8 * e + 4 * half + q4;
-      const int chunk = (dt * 4 + cq) ^ kv_swizzle<HD>(row);
+      const int chunk = (dt * 4 + cq) ^ row_swizzle<HD>(row);
       const unsigned char* a = v + (t * 32 + kk * 16 + row) * kRowB + chunk * 16 + lo8;
       const shortx4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4*)(a));
       part[e] = __builtin_bit_cast(uint2, r);
@@ -250,7 +245,7 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
         for (int e = 0; e < 16; e += 4) {
           __builtin_amdgcn_sched_barrier(0);
           const int d = dt * 32 + acc_row(e, half);
-          const uint2 x = *reinterpret_cast<const uint2*>(v + j * kRowB + (((d >> 3) ^ kv_swizzle<HD>(j & 15)) * 16) + (d & 4) * 2);
+          const uint2 x = *reinterpret_cast<const uint2*>(v + j * kRowB + (((d >> 3) ^ row_swizzle<HD>(j & 15)) * 16) + (d & 4) * 2);
           const uint32_t word[2] = {x.x, x.y};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -313,7 +308,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
 #pragma unroll
   for (int j = 0; j < HD / 32; ++j) {
     const int rr = (64 / CPR) * j + lane / CPR;
-    dma[j] = rr * row_bytes + (((lane & (CPR - 1)) ^ kv_swizzle<HD>(rr)) * 16);
+    dma[j] = rr * row_bytes + (((lane & (CPR - 1)) ^ row_swizzle<HD>(rr)) * 16);
   }
   const int64_t page_bytes = 2ll * p.page_size * row_bytes;
   const char* kvh = reinterpret_cast<const char*>(p.kv) + (int64_t)h * kRowB;
@@ -562,6 +557,7 @@ int check_chunk_args(const char* fn, const void* q, const void* kv_cache, const 
   if (int st = check_first_page_offset(fn, first_page_offset, page_size)) return st;
   if (nnz < 0) return fail(KIN_ERR_BAD_SHAPE, "%s: nnz=%lld is negative", fn, (long long)nnz);
   if (nnz * num_q_heads > 0x7fffffffLL / 2) return fail(KIN_ERR_UNSUPPORTED, "%s: nnz*num_q_heads is too large", fn);
+  if (num_q_heads > 32768) return fail(KIN_ERR_UNSUPPORTED, "%s: num_q_heads=%d is too many", fn, num_q_heads);
   if (num_pages < 1) return fail(KIN_ERR_BAD_SHAPE, "%s: num_pages=%lld must be >= 1", fn, (long long)num_pages);
   if (max_pages_per_seq < 1)
     return fail(KIN_ERR_BAD_SHAPE, "%s: max_pages_per_seq=%d must be >= 1", fn, max_pages_per_seq);

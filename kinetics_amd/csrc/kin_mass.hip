@@ -4,15 +4,16 @@
 // with the scores s of kin_chunk.h and the log-sum-exp that the attention over the same chunk wrote.
 //
 // A workgroup owns 128 tokens of one (sequence, KV head), each of its 4 waves 32 of them: their keys are read
-// once and stay in registers as the matrix unit's operand, and the rows pass by 32 at a time (they come
-// from L2).  S = Q K^T on v_mfma_f32_32x32x16 leaves lane l the scores of ONE token (column l % 32) against
+// once and stay in registers as the matrix unit's operand, and the rows pass by, 64 at a time, through two
+// stages in LDS that all four waves read.  S = Q K^T on v_mfma_f32_32x32x16 leaves lane l the scores of ONE token (column l % 32) against
 // 16 rows, so the sum over rows is a sum over registers: no atomics, one owner per token, and the order of
 // the additions never changes.  One exponential per (row, token): with many rows that is what bounds it.
 #include "kin_chunk.h"
 
 namespace kin {
 
-constexpr int kMassKeys = 128;
+constexpr int kMassKeys = 128;  // tokens of a workgroup
+constexpr int kMassRows = 64;   // rows of a staged tile (one per lane of a wave)
 
 struct MassParams {
   ChunkParams c;
@@ -25,7 +26,12 @@ struct MassParams {
 
 template <int HD, bool F16, bool EXTRA>
 __global__ __launch_bounds__(256, 2) void attention_mass_kernel(MassParams mp) {
-  __shared__ __attribute__((aligned(16))) float sm[4][3][32];
+  constexpr int kRowB = HD * 2;
+  constexpr int kStageB = kMassRows * kRowB;
+  constexpr int CPR = HD / 8, kLoads = kMassRows * CPR / 256;  // LDS-direct loads per wave and stage
+  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kStageB];
+  __shared__ __attribute__((aligned(16))) float lse_sh[2][kMassRows], slope_sh[2][kMassRows];
+  __shared__ __attribute__((aligned(16))) int hi_sh[2][kMassRows];
   const ChunkParams& p = mp.c;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -37,78 +43,139 @@ __global__ __launch_bounds__(256, 2) void attention_mass_kernel(MassParams mp) {
   const ChunkSeq sq = chunk_seq(p, b);
   if (sq.n == 0 || sq.len > mp.stride) return;
   const int rows = sq.n * p.group, off = p.first_page_offset, end = sq.len + off;
-  float* lse_sh = sm[wave][0];
-  int* hi_sh = reinterpret_cast<int*>(sm[wave][1]);
-  float* slope_sh = sm[wave][2];
+  const int base = sq.len - sq.n;  // position of the first row
   float* dst = mp.scores + ((int64_t)blk * p.hkv + h) * mp.stride;
+  const char* qh = reinterpret_cast<const char*>(p.q) + ((int64_t)sq.e0 * p.hq + h * p.group) * kRowB;
+  const int tok_bytes = p.hq * kRowB;
 
   for (int tile = rest % mp.key_tiles; tile * kMassKeys < end; tile += mp.key_tiles) {
-    const int slot0 = tile * kMassKeys + wave * 32;  // first token slot of the wave
-    if (slot0 >= end) continue;
+    const int wg_slot0 = tile * kMassKeys;
+    const int slot0 = wg_slot0 + wave * 32;  // first token slot of the wave
     const int slot = slot0 + col;
     // this lane's key: chunk 2k + half of its row for step k
     uint4 key[HD / 16];
     int id = -1;
     if (slot < end && slot >= off) id = sq.pages[slot >> p.page_shift];
     const bool ok = id >= 0 && (int64_t)id < p.num_pages;
-    const int64_t row = ((int64_t)(ok ? id : 0) * 2 * p.page_size + (slot & (p.page_size - 1))) * p.hkv + h;
-    const uint4* src = reinterpret_cast<const uint4*>(p.kv + row * HD);
+    const int64_t krow = ((int64_t)(ok ? id : 0) * 2 * p.page_size + (slot & (p.page_size - 1))) * p.hkv + h;
+    const uint4* src = reinterpret_cast<const uint4*>(p.kv + krow * HD);
 #pragma unroll
     for (int k = 0; k < HD / 16; ++k) key[k] = ok ? src[2 * k + half] : uint4{0, 0, 0, 0};
+    const bool all_keys = __ballot(!ok) == 0;
 
-    // rows that can see one of the wave's tokens: all of them below the prefix, else from the first token's own position to
-    // the end of the last one's window
-    const int base = sq.len - sq.n;
+    // rows that can see one of the workgroup's tokens: all of them below the prefix, else from the first token's own position
+    // to the end of the last one's window; rows in front of the sequence see nothing
     int i0 = 0, i1 = sq.n;
-    if (slot0 >= sq.prefix + off) {
-      i0 = max(slot0 - off - base, 0);
-      if (p.window > 0) i1 = (int)min((int64_t)sq.n, (int64_t)(slot0 + 31 - off) + p.window - base);
+    if (wg_slot0 >= sq.prefix + off) {
+      i0 = max(wg_slot0 - off - base, 0);
+      if (p.window > 0) i1 = (int)min((int64_t)sq.n, (int64_t)(wg_slot0 + kMassKeys - 1 - off) + p.window - base);
     }
-    i0 = max(i0, -base);  // rows in front of the sequence see nothing
-    float sum = 0.f;
-    for (int r0 = i0 * p.group; r0 < i1 * p.group; r0 += 32) {
-      const int r = r0 + col;
-      const bool valid = r < rows;
-      const int i = valid ? r / p.group : 0, g = valid ? r - i * p.group : 0;
-      const int64_t hq = (int64_t)(sq.e0 + i) * p.hq + h * p.group + g;
-      const uint4* qs = reinterpret_cast<const uint4*>(p.q + hq * HD);
-      floatx16 s;
+    i0 = max(i0, -base);
+    const int first = i0 * p.group, n_stages = i1 > i0 ? ((i1 - i0) * p.group + kMassRows - 1) / kMassRows : 0;
+    const int last = min(i1 * p.group, rows);  // one past the last row to count
+
+    // Rows of a stage as (token, head): x = the head of the stage's first row plus the row, below 2^16 / 16, so that
+    // x / group is a product and a shift.
+    const uint32_t magic = 65536u / p.group + 1;
+    auto split = [&](int x, int& q, int& g) {
+      q = (int)((uint32_t)x * magic >> 16);
+      g = x - q * p.group;
+    };
+    // Stage `st`: 64 rows, swizzled; rows that do not count lie outside the descriptor's 1 GiB and read as zeros.
+    auto stage_rows = [&](int st) {
+      const int r0 = first + st * kMassRows;
+      const int i = r0 / p.group, g0 = r0 - i * p.group;
+      const u32x4 rs = rsrc_words(qh + (int64_t)i * tok_bytes, 0x40000000);
+      const uint32_t at = lds_offset(lds + (st & 1) * kStageB);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = 0.f;
-      uint4 a[HD / 16];
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k) a[k] = valid ? qs[2 * k + half] : uint4{0, 0, 0, 0};
-      float z = valid ? mp.lse[hq] * kLog2e : INFINITY;
+      for (int j = 0; j < kLoads; ++j) {
+        const int rr = (wave * kLoads + j) * (64 / CPR) + lane / CPR;  // row of the stage
+        int di, g;
+        split(g0 + rr, di, g);
+        const int o = di * tok_bytes + g * kRowB + (((lane & (CPR - 1)) ^ row_swizzle<HD>(rr & 15)) * 16);
+        lds_load_16<false>(rs, at + (wave * kLoads + j) * 1024, r0 + rr < last ? o : 0x7fff0000);
+      }
+    };
+    // its rows' log-sum-exp (log2), token slots and slopes: one row per thread of the first wave
+    float z = 0.f, sl = 0.f;
+    int hi = 0;
+    auto fetch_row = [&](int st) {
+      const int r0 = first + st * kMassRows, i0s = r0 / p.group;
+      int di, g;
+      split(r0 - i0s * p.group + lane, di, g);
+      const int i = i0s + di;
+      const bool valid = r0 + lane < last;
+      z = valid ? mp.lse[(int64_t)(sq.e0 + i) * p.hq + h * p.group + g] * kLog2e : INFINITY;
       if (z == kNegInf) z = INFINITY;  // a row that saw nothing gives nothing
-      if (half == 0) {
-        lse_sh[col] = z;
-        hi_sh[col] = base + i + off;
-        if constexpr (EXTRA) slope_sh[col] = (p.slopes && valid) ? p.slopes[h * p.group + g] * kLog2e : 0.f;
+      hi = base + i + off;
+      if constexpr (EXTRA) sl = (p.slopes && valid) ? p.slopes[h * p.group + g] * kLog2e : 0.f;
+    };
+    auto put_row = [&](int st) {
+      lse_sh[st & 1][lane] = z;
+      hi_sh[st & 1][lane] = hi;
+      if constexpr (EXTRA) slope_sh[st & 1][lane] = sl;
+    };
+
+    float sum = 0.f;
+    if (n_stages > 0) {
+      stage_rows(0);
+      if (wave == 0) {
+        fetch_row(0);
+        put_row(0);
       }
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k) s = mfma_32x32x16<F16>(a[k], key[k], s);
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int rr = acc_row(e, half);
-        const float4 z4 = *reinterpret_cast<const float4*>(lse_sh + rr);
-        const int4 h4 = *reinterpret_cast<const int4*>(hi_sh + rr);
-        const float zz[4] = {z4.x, z4.y, z4.z, z4.w};
-        const int hh[4] = {h4.x, h4.y, h4.z, h4.w};
-        float sl[4] = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (EXTRA) {
-          const float4 s4 = *reinterpret_cast<const float4*>(slope_sh + rr);
-          sl[0] = s4.x; sl[1] = s4.y; sl[2] = s4.z; sl[3] = s4.w;
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float y = EXTRA ? chunk_score(p, s[e + x], sl[x], abs(hh[x] - slot)) - zz[x] : fmaf(s[e + x], p.scale_log2, -zz[x]);
-          const bool on = ok & (((slot <= hh[x]) & ((p.window == 0) | (hh[x] - slot < p.window))) | (slot < sq.prefix + off));
-          sum += on ? fast_exp2(y) : 0.f;
-        }
-      }
-      __builtin_amdgcn_wave_barrier();
     }
+    for (int st = 0; st < n_stages; ++st) {
+      __builtin_amdgcn_s_waitcnt(0);  // this wave's part of the stage is in; behind the barrier, every wave's
+      __syncthreads();
+      const bool more = st + 1 < n_stages;
+      if (more) {
+        stage_rows(st + 1);
+        if (wave == 0) fetch_row(st + 1);
+      }
+      const unsigned char* qs = lds + (st & 1) * kStageB;
+#pragma unroll
+      for (int t = 0; t < kMassRows / 32; ++t) {
+        const int r0 = first + st * kMassRows + t * 32;
+        const int pos0 = base + r0 / p.group, pos1 = base + min(r0 + 31, last - 1) / p.group;
+        if (r0 >= last || slot0 >= end) break;
+        if (slot0 >= sq.prefix + off && slot0 - off > pos1) continue;  // behind all of these rows
+        floatx16 s;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint4 a = *reinterpret_cast<const uint4*>(qs + (t * 32 + col) * kRowB + (((2 * k + half) ^ row_swizzle<HD>(col & 15)) * 16));
+          s = mfma_32x32x16<F16>(a, key[k], s);
+        }
+        const bool seen = all_keys && ((slot0 + 31 - off <= pos0 && (p.window == 0 || pos1 - (slot0 - off) < p.window)) ||
+                                       slot0 + 31 < sq.prefix + off);
+        const float* zs = lse_sh[st & 1] + t * 32;
+        const int* hs = hi_sh[st & 1] + t * 32;
+        if constexpr (EXTRA) {
+          cap_scores(p, s);
+          if (p.slopes) {
+            const float* ss = slope_sh[st & 1] + t * 32;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = fmaf(-ss[acc_row(e, half)], (float)abs(hs[acc_row(e, half)] - slot), s[e]);
+          }
+        }
+        const float c = EXTRA ? 1.f : p.scale_log2;
+        if (!seen) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int at = hs[acc_row(e, half)];
+            const bool on = ok & (((slot <= at) & ((p.window == 0) | (at - slot < p.window))) | (slot < sq.prefix + off));
+            s[e] = on ? s[e] : kNegInf;
+          }
+        }
+        float part = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) part += fast_exp2(fmaf(s[e], c, -zs[acc_row(e, half)]));
+        sum += part;
+      }
+      if (more && wave == 0) put_row(st + 1);
+    }
+    __syncthreads();  // the staging area is free for the next tile of keys
     sum += other_half(sum);
     if (half == 0 && slot >= off && slot < end) dst[slot - off] += sum;
   }
