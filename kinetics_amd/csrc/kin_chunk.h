@@ -166,6 +166,11 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return (uint32_t)reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p);
 }
 
+// The larger of lane l's and lane l ^ 32's value (no LDS).
+__device__ __forceinline__ float max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 // The value of lane ^ 32.
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
 

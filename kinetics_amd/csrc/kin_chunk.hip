@@ -68,6 +68,7 @@ struct WaveRows {
   float m, l;       // running maximum (units of the raw product, or log2 with EXTRA) and this lane's part of the sum
   RowSpan span;
   float slope2;
+  uint64_t pos_inf, neg_inf;  // bit e: output register e gets an infinity of that sign (both: NaN)
 };
 
 template <int HD>
@@ -76,6 +77,7 @@ __device__ __forceinline__ void load_rows(const ChunkParams& p, const ChunkSeq& 
   const int i = r / p.group, g = r - i * p.group;
   w.m = kNegInf;
   w.l = 0.f;
+  w.pos_inf = w.neg_inf = 0;
 #pragma unroll
   for (int t = 0; t < HD / 32; ++t)
 #pragma unroll
@@ -156,7 +158,7 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
   for (int t = 0; t < NSUB; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[t][e]);
-  mt = fmaxf(mt, other_half(mt));
+  mt = max_halves(mt);
   // The reference maximum follows the scores only when they pass it by 2^8 (weights stay below 2^8, which both
   // element types and the fp32 sums hold without loss), so most blocks need no rescaling of O.
   const bool move = mt > w.m && !((mt - w.m) * c <= kRescaleLog2);
@@ -200,59 +202,57 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
     }
     return uint4{part[0].x, part[0].y, part[1].x, part[1].y};
   };
-  bool special = false;
-  if (masked) {
-    bool any = false;
+#pragma unroll
+  for (int t = 0; t < NSUB; ++t)
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int dt = 0; dt < HD / 32; ++dt) w.o[dt] = mfma_32x32x16<F16>(read_v(t, kk, dt), pb[t][kk], w.o[dt]);
+}
+
+// A value that is not seen has weight 0, and 0 times an infinity would be NaN.  In the blocks where some row does not see
+// some key, infinite and NaN values are therefore taken out of the staged rows: which elements of this
+// lane's output they reach is kept as bits, and the result gets them at the end.
+template <int HD, bool F16>
+__device__ __forceinline__ bool rows_special(const unsigned char* v, int rows) {
+  bool any = false;
 #pragma unroll 1
-    for (int x = lane; x < NSUB * 32 * (HD / 8); x += 64) any |= any_special<F16>(*reinterpret_cast<const uint4*>(v + x * 16));
-    special = __ballot(any) != 0;
-  }
-  if (!special) {
-#pragma unroll
-    for (int t = 0; t < NSUB; ++t)
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int dt = 0; dt < HD / 32; ++dt) w.o[dt] = mfma_32x32x16<F16>(read_v(t, kk, dt), pb[t][kk], w.o[dt]);
-  } else {
-    // Some value of the block is infinite or NaN (rare).  One that is not seen has weight 0, and 0 times an infinity
-    // would be NaN: the product takes the finite values only, and the others are added to the rows that see them.
-#pragma unroll
-    for (int t = 0; t < NSUB; ++t)
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-        for (int dt = 0; dt < HD / 32; ++dt) {
-          __builtin_amdgcn_sched_barrier(0);
-          w.o[dt] = mfma_32x32x16<F16>(finite_only<F16>(read_v(t, kk, dt)), pb[t][kk], w.o[dt]);
-        }
-    uint64_t sees = 0;  // bit j: this lane's row gives key j a weight
-#pragma unroll
-    for (int t = 0; t < NSUB; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const uint4 d = pb[t][e >> 3];
-        const uint32_t word = ((e >> 1) & 3) == 0 ? d.x : (((e >> 1) & 3) == 1 ? d.y : (((e >> 1) & 3) == 2 ? d.z : d.w));
-        sees |= (uint64_t)(((word >> (16 * (e & 1))) & 0x7fffu) ? 1 : 0) << (t * 32 + acc_row(e, half));
+  for (int x = threadIdx.x & 63; x < rows * (HD / 8); x += 64) any |= any_special<F16>(*reinterpret_cast<const uint4*>(v + x * 16));
+  return __ballot(any) != 0;
+}
+template <int HD, bool F16>
+__device__ __forceinline__ void note_specials(WaveRows<HD>& w, const unsigned char* v, int keys, int slot0, uint32_t units, int first) {
+  const int half = (threadIdx.x >> 5) & 1;
+#pragma unroll 1
+  for (int j = 0; j < keys; ++j) {
+    const bool on = row_sees(w.span, first, slot0 + j) && ((units >> (j >> 4)) & 1);
+#pragma unroll 1
+    for (int x = 0; x < HD / 2; ++x) {  // element x % 16 of output tile x / 16
+      const int d = (x >> 4) * 32 + acc_row(x & 15, half);
+      const uint32_t bits = *reinterpret_cast<const uint16_t*>(v + j * HD * 2 + (((d >> 3) ^ row_swizzle<HD>(j & 15)) * 16) + (d & 7) * 2);
+      const float y = elem_lo<F16>(bits);
+      if (on && !(fabsf(y) < INFINITY)) {
+        if (!(y < 0.f)) w.pos_inf |= 1ull << x;
+        if (!(y > 0.f)) w.neg_inf |= 1ull << x;
       }
-    sees |= __shfl_xor(sees, 32);
+    }
+  }
+}
+template <int HD, bool F16>
+__device__ __forceinline__ void clear_specials(unsigned char* v, int rows) {
 #pragma unroll 1
-    for (int j = 0; j < NSUB * 32; ++j) {
-      const bool on = (sees >> j) & 1;
+  for (int x = threadIdx.x & 63; x < rows * (HD / 8); x += 64) {
+    uint4* at = reinterpret_cast<uint4*>(v + x * 16);
+    *at = finite_only<F16>(*at);
+  }
+}
+template <int HD>
+__device__ __forceinline__ void put_specials(WaveRows<HD>& w) {
+  if (__ballot((w.pos_inf | w.neg_inf) != 0)) {
 #pragma unroll
-      for (int dt = 0; dt < HD / 32; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          __builtin_amdgcn_sched_barrier(0);
-          const int d = dt * 32 + acc_row(e, half);
-          const uint2 x = *reinterpret_cast<const uint2*>(v + j * kRowB + (((d >> 3) ^ row_swizzle<HD>(j & 15)) * 16) + (d & 4) * 2);
-          const uint32_t word[2] = {x.x, x.y};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float y = i & 1 ? elem_hi<F16>(word[i >> 1]) : elem_lo<F16>(word[i >> 1]);
-            w.o[dt][e + i] += on && !(fabsf(y) < INFINITY) ? y : 0.f;
-          }
-        }
+    for (int x = 0; x < HD / 2; ++x) {
+      if ((w.pos_inf >> x) & 1) w.o[x >> 4][x & 15] += INFINITY;
+      if ((w.neg_inf >> x) & 1) w.o[x >> 4][x & 15] -= INFINITY;
     }
   }
 }
@@ -312,11 +312,9 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
   }
   const int64_t page_bytes = 2ll * p.page_size * row_bytes;
   const char* kvh = reinterpret_cast<const char*>(p.kv) + (int64_t)h * kRowB;
-  const __attribute__((address_space(4))) int32_t* pages =
-      reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(sq.pages));
-  auto page_of = [&](int unit) -> int {  // page id of the 16 token slots `unit`; -1 outside the cache
-    const int i = (unit * 16) >> p.page_shift;
-    const int id = pages[min(i, sq.n_pages - 1)];
+  // Page id of the 16 token slots `unit`; -1 outside the cache.  Ids are fetched a whole batch of blocks ahead, one per lane.
+  auto page_of = [&](int unit) -> int {
+    const int id = sq.pages[min((unit * 16) >> p.page_shift, sq.n_pages - 1)];
     return (id >= 0 && (int64_t)id < p.num_pages) ? id : -1;
   };
   // Descriptors of a unit's K and V rows; token slots behind the sequence read as zeros, whatever the page holds there.
@@ -339,28 +337,37 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
 
   if (narrow) {
     // Blocks of 32 token slots of the tiles it0 .. it1-1, every fourth one for this wave.
-    const int n_blocks = 2 * (it1 - it0);
+    const int n_blocks = (2 * (it1 - it0) - wave + 3) >> 2;
     unsigned char* kbuf = lds + wave * kWaveB;
     unsigned char* vbuf = kbuf + 32 * kRowB;
-    auto unit_at = [&](int i) { return tile_at(it0 + (i >> 1)) * 4 + (i & 1) * 2; };
-    int id0 = -1, id1 = -1;
-    if (wave < n_blocks) {
-      const int u = unit_at(wave);
-      id0 = page_of(u);
-      id1 = page_of(u + 1);
+    auto unit_at = [&](int x) {  // first unit of the wave's block x (the last one's behind the end)
+      const int i = wave + 4 * min(x, n_blocks - 1);
+      return tile_at(it0 + (i >> 1)) * 4 + (i & 1) * 2;
+    };
+    auto fetch_ids = [&](int x) { return page_of(unit_at(x + (lane >> 1)) + (lane & 1)); };
+    int ids = -1, ids_next = -1, id0 = -1, id1 = -1;
+    if (n_blocks > 0) {
+      ids = fetch_ids(0);
+      if (n_blocks > 31) ids_next = fetch_ids(32);
+      id0 = __builtin_amdgcn_readlane(ids, 0);
+      id1 = __builtin_amdgcn_readlane(ids, 1);
+      const int u = unit_at(0);
       stage_unit(unit_rsrc(u, id0, false), kbuf, true);
       stage_unit(unit_rsrc(u + 1, id1, false), kbuf + kUnitB, true);
       stage_unit(unit_rsrc(u, id0, true), vbuf, true);
       stage_unit(unit_rsrc(u + 1, id1, true), vbuf + kUnitB, true);
     }
-    for (int i = wave; i < n_blocks; i += 4) {
-      const int u = unit_at(i);
+    for (int x = 0; x < n_blocks; ++x) {
+      const int u = unit_at(x);
       const uint32_t units = (id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u);
       // the next block (behind the last one: empty descriptors, so that the counts below hold)
-      const bool more = i + 4 < n_blocks;
-      const int un = more ? unit_at(i + 4) : u;
-      int n0 = page_of(un), n1 = page_of(un + 1);
-      if (!more) n0 = n1 = -1;
+      if (((x + 1) & 31) == 0) {
+        ids = ids_next;
+        if (x + 33 < n_blocks) ids_next = fetch_ids(x + 33);
+      }
+      int n0 = __builtin_amdgcn_readlane(ids, 2 * ((x + 1) & 31)), n1 = __builtin_amdgcn_readlane(ids, 2 * ((x + 1) & 31) + 1);
+      if (x + 1 >= n_blocks) n0 = n1 = -1;
+      const int un = unit_at(x + 1);
       const int slot0 = u * 16;
       const bool all = slot0 >= (p.window > 0 ? max(pos1 - p.window + 1, 0) : 0) + off && slot0 + 31 <= pos0 + off;
       const bool masked = !(units == 3u && (all || (slot0 >= off && slot0 + 32 <= sq.prefix + off && pos0 >= 0)));
@@ -378,6 +385,10 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(wait_vm_imm(HD / 16));  // the values are in; the next keys may be on their way
         __builtin_amdgcn_sched_barrier(0);
+        if (masked && rows_special<HD, F16>(vbuf, 32)) {
+          note_specials<HD, F16>(w, vbuf, 32, slot0, units, off);
+          clear_specials<HD, F16>(vbuf, 32);
+        }
       };
       attend_block<HD, F16, EXTRA, 1>(p, w, kbuf, vbuf, slot0, masked, units, after_k, before_v);
       __builtin_amdgcn_sched_barrier(0);
@@ -388,6 +399,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
       id0 = n0;
       id1 = n1;
     }
+    put_specials<HD>(w);
     __builtin_amdgcn_s_waitcnt(0);
     // Join the waves: every wave leaves its rows' maxima, sums and outputs in LDS.
     w.l += other_half(w.l);
@@ -449,39 +461,57 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
   const bool mine = wave * 32 < nrows;
   const int wpos0 = sq.len - sq.n + (r0 + wave * 32) / p.group;
   const int wpos1 = sq.len - sq.n + (r0 + min(wave * 32 + 31, nrows - 1)) / p.group;
+  auto fetch_ids = [&](int it) { return page_of(tile_at(min(it + (lane >> 2), it1 - 1)) * 4 + (lane & 3)); };  // 16 tiles
+  int ids = -1, ids_next = -1;
   auto stage_tile = [&](int it, unsigned char* dst, uint32_t& units) {
-    const int u0 = tile_at(it) * 4;
-    uint32_t ok = 0;
-    int id = -1;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int x = page_of(u0 + k);
-      ok |= x >= 0 ? 1u << k : 0u;
-      if (k == wave) id = x;
+    const int k = (it - it0) & 15;
+    if (k == 0) {
+      ids = ids_next;
+      if (it + 16 < it1) ids_next = fetch_ids(it + 16);
     }
-    units = ok;
-    stage_unit(unit_rsrc(u0 + wave, id, false), dst + wave * kUnitB, false);
-    stage_unit(unit_rsrc(u0 + wave, id, true), dst + (4 + wave) * kUnitB, false);
+    units = (uint32_t)(__ballot(ids >= 0) >> (4 * k)) & 15u;
+    const int id = __builtin_amdgcn_readlane(ids, 4 * k + wave);
+    const int u = tile_at(it) * 4 + wave;
+    stage_unit(unit_rsrc(u, id, false), dst + wave * kUnitB, false);
+    stage_unit(unit_rsrc(u, id, true), dst + (4 + wave) * kUnitB, false);
   };
   uint32_t units_next = 0;
-  if (it0 < it1) stage_tile(it0, lds, units_next);
+  if (it0 < it1) {
+    ids_next = fetch_ids(it0);
+    stage_tile(it0, lds, units_next);
+  }
+  // No row of [rows at first .. last position] misses a key of the tile.
+  auto seen_whole = [&](int slot0, uint32_t units, int first, int last) {
+    const bool causal = slot0 >= (p.window > 0 ? max(last - p.window + 1, 0) : 0) + off && slot0 + kChunkKeys - 1 <= first + off;
+    return units == 15u && (causal || (slot0 >= off && slot0 + kChunkKeys <= sq.prefix + off && first >= 0));
+  };
   for (int it = it0; it < it1; ++it) {
     const int stage = (it - it0) & 1;
     const uint32_t units = units_next;
+    unsigned char* kst = lds + stage * kStageB;
+    unsigned char* vst = kst + kChunkKeys * kRowB;
     __builtin_amdgcn_s_waitcnt(0);  // this wave's part of the tile is in; behind the barrier, every wave's
     __syncthreads();
     if (it + 1 < it1) stage_tile(it + 1, lds + (1 - stage) * kStageB, units_next);
     const int slot0 = tile_at(it) * kChunkKeys;
+    if (!seen_whole(slot0, units, pos0, pos1)) {  // the whole workgroup looks for infinite and NaN values
+      const bool any = rows_special<HD, F16>(vst + wave * kUnitB, 16);
+      if (lane == 0) sm_m[0][wave] = any ? 1.f : 0.f;
+      __syncthreads();
+      if (sm_m[0][0] + sm_m[0][1] + sm_m[0][2] + sm_m[0][3] > 0.f) {
+        if (mine) note_specials<HD, F16>(w, vst, kChunkKeys, slot0, units, off);
+        __syncthreads();
+        clear_specials<HD, F16>(vst + wave * kUnitB, 16);
+        __syncthreads();
+      }
+    }
     if (!mine) continue;
     const bool in_prefix = slot0 < sq.prefix + off;
     if (!in_prefix && (slot0 > wpos1 + off || (p.window > 0 && slot0 + kChunkKeys <= wpos0 - p.window + 1 + off))) continue;
-    const bool all = slot0 >= (p.window > 0 ? max(wpos1 - p.window + 1, 0) : 0) + off && slot0 + kChunkKeys - 1 <= wpos0 + off;
-    const bool masked = !(units == 15u && (all || (slot0 >= off && slot0 + kChunkKeys <= sq.prefix + off && wpos0 >= 0)));
-    const unsigned char* kst = lds + stage * kStageB;
-    const unsigned char* vst = kst + kChunkKeys * kRowB;
     auto nothing = []() {};
-    attend_block<HD, F16, EXTRA, 2>(p, w, kst, vst, slot0, masked, units, nothing, nothing);
+    attend_block<HD, F16, EXTRA, 2>(p, w, kst, vst, slot0, !seen_whole(slot0, units, wpos0, wpos1), units, nothing, nothing);
   }
+  put_specials<HD>(w);
   if (row < nrows) {
     const float c = EXTRA ? 1.f : p.scale_log2;
     const float l = w.l + other_half(w.l);
