@@ -49,17 +49,21 @@ struct ChunkSeq {
   const int32_t* pages;
 };
 
-__device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int b) {
+// From the raw table entries of one sequence.
+__device__ __forceinline__ ChunkSeq make_chunk_seq(const ChunkParams& p, int e0, int e1, int ps, int pe, int last, int prefix) {
   ChunkSeq s;
-  s.e0 = min(max(p.q_indptr[b], 0), p.nnz);
-  s.n = min(max(p.q_indptr[b + 1], s.e0), p.nnz) - s.e0;
-  const int ps = p.page_indptr[b];
-  s.n_pages = max(p.page_indptr[b + 1] - ps, 0);
+  s.e0 = min(max(e0, 0), p.nnz);
+  s.n = min(max(e1, s.e0), p.nnz) - s.e0;
+  s.n_pages = max(pe - ps, 0);
   s.pages = p.page_indices + ps;
-  const int last = min(max(p.last_page_len[b], 0), p.page_size);
+  last = min(max(last, 0), p.page_size);
   s.len = s.n_pages > 0 ? max((s.n_pages - 1) * p.page_size + last - p.first_page_offset, 0) : 0;
-  s.prefix = p.prefix_lens ? min(max(p.prefix_lens[b], 0), s.len) : 0;
+  s.prefix = min(max(prefix, 0), s.len);
   return s;
+}
+__device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams& p, int b) {
+  return make_chunk_seq(p, p.q_indptr[b], p.q_indptr[b + 1], p.page_indptr[b], p.page_indptr[b + 1], p.last_page_len[b],
+                        p.prefix_lens ? p.prefix_lens[b] : 0);
 }
 
 // The token slots (tokens shifted by the first page's padding) that one row sees:

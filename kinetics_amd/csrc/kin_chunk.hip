@@ -37,27 +37,40 @@ struct ChunkAttnParams {
 
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 
-// First row tile of sequence b: tiles are numbered so that every sequence has room for its rows
-// whatever the others bring, without a scan: floor(q_indptr[b] * group / 128) + b.
-__device__ __forceinline__ int first_slot(const ChunkParams& p, int b) {
-  return (int)((int64_t)min(max(p.q_indptr[b], 0), p.nnz) * p.group / kChunkRows) + b;
+// First row tile of the sequence b whose rows start at e0: tiles are numbered so that every sequence has room for its rows
+// whatever the others bring, without a scan: floor(e0 * group / 128) + b.
+__device__ __forceinline__ int first_slot(const ChunkParams& p, int e0, int b) {
+  return (int)((int64_t)e0 * p.group / kChunkRows) + b;
 }
-// The sequence that owns row tile `slot`: the last one whose first tile is not behind it (64 candidates
-// per step).  -1 if there is none.
-__device__ __forceinline__ int seq_of_slot(const ChunkParams& p, int slot) {
+__device__ __forceinline__ int first_row(const ChunkParams& p, int b) { return min(max(p.q_indptr[b], 0), p.nnz); }
+// The sequence that owns row tile `slot` -- the last one whose first tile is not behind it -- into sq; -1 if there is none.
+__device__ __forceinline__ int seq_of_slot(const ChunkParams& p, int slot, ChunkSeq& sq) {
   const int lane = threadIdx.x & 63;
+  if (p.batch <= 64) {  // one sequence per lane: everything about it in one round trip
+    const int i = min(lane, p.batch - 1);
+    const int e0 = first_row(p, i), e1 = p.q_indptr[i + 1], ps = p.page_indptr[i], pe = p.page_indptr[i + 1];
+    const int last = p.last_page_len[i], prefix = p.prefix_lens ? p.prefix_lens[i] : 0;
+    const int b = __popcll(__ballot(lane < p.batch && first_slot(p, e0, i) <= slot)) - 1;
+    if (b < 0) return -1;
+    sq = make_chunk_seq(p, __builtin_amdgcn_readlane(e0, b), __builtin_amdgcn_readlane(e1, b), __builtin_amdgcn_readlane(ps, b),
+                        __builtin_amdgcn_readlane(pe, b), __builtin_amdgcn_readlane(last, b), __builtin_amdgcn_readlane(prefix, b));
+    return b;
+  }
   int lo = 0, n = p.batch;
-  while (true) {
+  while (true) {  // 64 candidates per step
     const int step = (n + 63) >> 6;
     const int b = lo + lane * step;
-    const bool ok = b < lo + n && first_slot(p, b) <= slot;
+    const bool ok = b < lo + n && first_slot(p, first_row(p, b), b) <= slot;
     const int count = __popcll(__ballot(ok));
     if (count == 0) return -1;
     const int next = lo + (count - 1) * step;
     n = min(step, lo + n - next);
     lo = next;
-    if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
+    if (step == 1) break;
   }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  sq = chunk_seq(p, lo);
+  return lo;
 }
 
 // One wave's 32 rows: queries as a matrix operand, running softmax, output.
@@ -273,11 +286,11 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
   const int h = blockIdx.x % p.hkv;
   const int slot = ap.slots - 1 - (int)(blockIdx.x / p.hkv);  // the later rows of a sequence see more keys: they go first
   const int split = blockIdx.y;
-  const int b = seq_of_slot(p, slot);
+  ChunkSeq sq;
+  const int b = seq_of_slot(p, slot, sq);
   if (b < 0) return;
-  const ChunkSeq sq = chunk_seq(p, b);
   const int rows = sq.n * p.group;   // int: nnz * group is checked on the host
-  const int r0 = (slot - first_slot(p, b)) * kChunkRows;
+  const int r0 = (slot - first_slot(p, sq.e0, b)) * kChunkRows;
   if (r0 >= rows) return;
   const int nrows = min(rows - r0, kChunkRows);
   const bool narrow = nrows <= 32;   // uniform
@@ -543,29 +556,62 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
   }
 }
 
-// Joins the spans of the keys: HD / 4 lanes per (row, query head).  Rows that belong to no sequence are left alone.
-template <int HD, bool F16>
+// Joins the spans of the keys: HD / 4 lanes per (row, query head), GROUPS of them sharing its spans (few rows have many spans, and
+// reading those one after the other is all latency: 16 spans of 32 rows 7.3 us with one group).
+// Rows that belong to no sequence are left alone.
+template <int HD, bool F16, int GROUPS>
 __global__ __launch_bounds__(256) void merge_chunk_kernel(ChunkAttnParams ap) {
-  constexpr int LPR = HD / 4;
+  constexpr int LPR = HD / 4, ROWS = 256 / (LPR * GROUPS);
+  __shared__ float sm_m[GROUPS][ROWS], sm_l[GROUPS][ROWS];
+  __shared__ __attribute__((aligned(16))) float sm_o[GROUPS][ROWS][HD];
   const int64_t total = (int64_t)ap.c.nnz * ap.c.hq;
-  const int64_t x = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int d = (threadIdx.x % LPR) * 4, g = threadIdx.x / LPR % GROUPS, r = threadIdx.x / (LPR * GROUPS);
+  const int64_t x = (int64_t)blockIdx.x * ROWS + r;
   const int64_t tok = x / ap.c.hq;
-  if (x >= total || tok < ap.c.q_indptr[0] || tok >= ap.c.q_indptr[ap.c.batch]) return;
-  const int d = (threadIdx.x % LPR) * 4;
-  float mm = kNegInf;
-  for (int s = 0; s < ap.num_splits; ++s) mm = fmaxf(mm, ap.ws_lse[s * total + x]);
-  const float safe = mm == kNegInf ? 0.f : mm;
-  float den = 0.f;
+  const bool mine = x < total && tok >= ap.c.q_indptr[0] && tok < ap.c.q_indptr[ap.c.batch];
+  float mm = kNegInf, den = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < ap.num_splits; ++s) {
-    const float f = fast_exp2(ap.ws_lse[s * total + x] - safe);
-    const float4 o = *reinterpret_cast<const float4*>(ap.ws_o + (s * total + x) * HD + d);
-    den += f;
-    acc.x = fmaf(f, o.x, acc.x);
-    acc.y = fmaf(f, o.y, acc.y);
-    acc.z = fmaf(f, o.z, acc.z);
-    acc.w = fmaf(f, o.w, acc.w);
+  if (mine) {
+#pragma unroll 8
+    for (int s = g; s < ap.num_splits; s += GROUPS) mm = fmaxf(mm, ap.ws_lse[s * total + x]);
+    const float safe = mm == kNegInf ? 0.f : mm;
+#pragma unroll 8
+    for (int s = g; s < ap.num_splits; s += GROUPS) {
+      const float f = fast_exp2(ap.ws_lse[s * total + x] - safe);
+      const float4 o = *reinterpret_cast<const float4*>(ap.ws_o + (s * total + x) * HD + d);
+      den += f;
+      acc.x = fmaf(f, o.x, acc.x);
+      acc.y = fmaf(f, o.y, acc.y);
+      acc.z = fmaf(f, o.z, acc.z);
+      acc.w = fmaf(f, o.w, acc.w);
+    }
   }
+  if constexpr (GROUPS > 1) {
+    if (d == 0) {
+      sm_m[g][r] = mm;
+      sm_l[g][r] = den;
+    }
+    *reinterpret_cast<float4*>(&sm_o[g][r][d]) = acc;
+    __syncthreads();
+    if (g > 0) return;
+    mm = kNegInf;
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) mm = fmaxf(mm, sm_m[k][r]);
+    const float safe = mm == kNegInf ? 0.f : mm;
+    den = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+      const float f = fast_exp2(sm_m[k][r] - safe);
+      const float4 o = *reinterpret_cast<const float4*>(&sm_o[k][r][d]);
+      den = fmaf(f, sm_l[k][r], den);
+      acc.x = fmaf(f, o.x, acc.x);
+      acc.y = fmaf(f, o.y, acc.y);
+      acc.z = fmaf(f, o.z, acc.z);
+      acc.w = fmaf(f, o.w, acc.w);
+    }
+  }
+  if (!mine) return;
   const bool none = mm == kNegInf && den == 0.f;
   const float inv = none ? 0.f : 1.f / den;
   uint2 y;
@@ -650,9 +696,13 @@ static void launch_chunk(const ChunkAttnParams& ap, dim3 grid, bool extra, hipSt
   if (extra) chunk_attn_kernel<HD, F16, true><<<grid, 256, 0, stream>>>(ap);
   else chunk_attn_kernel<HD, F16, false><<<grid, 256, 0, stream>>>(ap);
   if (ap.num_splits > 1) {
-    const int per = 256 / (HD / 4);
-    const unsigned g = (unsigned)(((int64_t)ap.c.nnz * ap.c.hq + per - 1) / per);
-    merge_chunk_kernel<HD, F16><<<g, 256, 0, stream>>>(ap);
+    const int64_t rows = (int64_t)ap.c.nnz * ap.c.hq;
+    if (ap.num_splits > 4) {
+      merge_chunk_kernel<HD, F16, 1024 / HD><<<(unsigned)rows, 256, 0, stream>>>(ap);
+    } else {
+      const int per = 1024 / HD;
+      merge_chunk_kernel<HD, F16, 1><<<(unsigned)((rows + per - 1) / per), 256, 0, stream>>>(ap);
+    }
   }
 }
 
