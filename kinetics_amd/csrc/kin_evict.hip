@@ -12,9 +12,11 @@
 namespace kin {
 
 constexpr int kEvictThreads = 1024;
-constexpr int kEvictPer = 4;        // tokens per lane and step of the ordered pass
-constexpr int kMoveThreads = 512;
-constexpr int kMoveRows = 4;        // rows per lane in flight
+constexpr int kEvictPer = 8;        // tokens per lane and step of the ordered pass
+constexpr int kDigitBits = 11;      // of the radix search: sign, exponent and two bits of the fraction come first, so that scores of
+constexpr int kDigits = 1 << kDigitBits;  // one size do not all count in one place (LDS atomics on one address queue up)
+constexpr int kMoveThreads = 1024;
+constexpr int kMoveRows = 8;        // rows per lane in flight: a stretch is 1024 rows, 128 KiB of registers
 
 struct EvictParams {
   uint16_t* kv;
@@ -54,8 +56,9 @@ __device__ __forceinline__ EvictSeq evict_seq(const EvictParams& p, int b) {
 }
 
 __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams p) {
-  __shared__ uint32_t hist[256];
+  __shared__ uint32_t hist[kDigits];
   __shared__ uint32_t pick[2];   // digit that holds the cut, keys above it
+  __shared__ uint32_t wave_above[kEvictThreads / 64];
   __shared__ int2 wave_sum[kEvictThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x / p.hkv, h = blockIdx.x - b * p.hkv;
@@ -77,39 +80,38 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams
       for (int i = tid; i < n; i += kEvictThreads) dst[i] = src[i];
     return;
   }
-  // The m-th largest key of the tokens sink .. n - local - 1, eight bits at a time.
+  // The m-th largest key of the tokens sink .. n - local - 1, a digit at a time from the top (11, 11, 10 bits).
   const int c0 = p.sink, c1 = n - p.local;
   uint32_t cut = 0, above = 0;
   if (m > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+    for (int top = 32; top > 0; top -= kDigitBits) {  // bits below `top` are still open
+      const int shift = max(top - kDigitBits, 0);
+      for (int d = tid; d < kDigits; d += kEvictThreads) hist[d] = 0;
       __syncthreads();
+#pragma unroll 8
       for (int i = c0 + tid; i < c1; i += kEvictThreads) {
         const uint32_t k = score_key(src[i]);
-        if (shift == 24 || (k >> (shift + 8)) == (cut >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1u);
+        if (top == 32 || (k >> top) == (cut >> top)) atomicAdd(&hist[(k >> shift) & ((1u << (top - shift)) - 1)], 1u);
       }
       __syncthreads();
-      if (wave == 0) {  // lane l sums the digits 255 - 4l .. 252 - 4l
-        uint32_t c[4], s = 0;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          c[x] = hist[255 - 4 * lane - x];
-          s += c[x];
-        }
-        uint32_t before = wave_inclusive_sum(s) - s + above;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if (before < (uint32_t)m && before + c[x] >= (uint32_t)m) {
-            pick[0] = 255 - 4 * lane - x;
-            pick[1] = before;
-          }
-          before += c[x];
-        }
+      // thread t holds the digits kDigits - 1 - 2t and the one below: how many keys lie above them?
+      const int d0 = kDigits - 1 - 2 * tid;
+      const uint32_t h0 = hist[d0], h1 = hist[d0 - 1];
+      const uint32_t incl = wave_inclusive_sum(h0 + h1);
+      if (lane == 63) wave_above[wave] = incl;
+      __syncthreads();
+      uint32_t before = above + incl - h0 - h1;
+      for (int w = 0; w < wave; ++w) before += wave_above[w];
+      if (before < (uint32_t)m && before + h0 >= (uint32_t)m) {
+        pick[0] = d0;
+        pick[1] = before;
+      } else if (before + h0 < (uint32_t)m && before + h0 + h1 >= (uint32_t)m) {
+        pick[0] = d0 - 1;
+        pick[1] = before + h0;
       }
       __syncthreads();
       cut |= pick[0] << shift;
       above = pick[1];
-      __syncthreads();
     }
   }
   const int ties = m - (int)above;  // tokens with the cut score itself that stay, from the lowest index on
@@ -178,32 +180,48 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p,
   const int64_t page_bytes = 2ll * p.page_size * row_bytes;
   char* base = reinterpret_cast<char*>(p.kv) + (int64_t)plane * p.page_size * row_bytes + (int64_t)h * (row_bytes / p.hkv) +
                part * 128 + (tid & 7) * 16;
-  auto row_of = [&](int token) -> char* {
+  // Row of the cache that holds a token (page * page_size + slot); none: its page is outside the cache.
+  constexpr uint32_t kNone = 0xffffffffu;
+  auto row_of = [&](int token) -> uint32_t {
     const int at = token + p.first_page_offset;
     const int id = sq.pages[at >> p.page_shift];
-    if (id < 0 || (int64_t)id >= p.num_pages) return nullptr;
-    return base + (int64_t)id * page_bytes + (int64_t)(at & (p.page_size - 1)) * row_bytes;
+    return id >= 0 && (int64_t)id < p.num_pages ? ((uint32_t)id << p.page_shift) + (at & (p.page_size - 1)) : kNone;
+  };
+  auto address = [&](uint32_t row) -> char* {
+    return base + (int64_t)(row >> p.page_shift) * page_bytes + (int64_t)(row & (p.page_size - 1)) * row_bytes;
   };
   constexpr int kStep = kMoveThreads / 8;
-  for (int first = p.sink; first < p.budget; first += kStep * kMoveRows) {
-    u32x4 v[kMoveRows];
-    char* to[kMoveRows];
+  uint32_t from[kMoveRows], to[kMoveRows];
+  auto find_rows = [&](int first) {
+    int src[kMoveRows];
 #pragma unroll
     for (int j = 0; j < kMoveRows; ++j) {
       const int dst = first + j * kStep + (tid >> 3);
-      const int src = dst < p.budget ? kept[dst] : dst;
-      to[j] = nullptr;
-      if (src != dst) {  // tokens in front of the first gap stay where they are
-        const char* from = row_of(src);
-        to[j] = from ? row_of(dst) : nullptr;
-        if (to[j]) v[j] = *reinterpret_cast<const u32x4*>(from);
-      }
+      src[j] = dst < p.budget ? kept[dst] : dst;
     }
-    __builtin_amdgcn_s_waitcnt(0);  // every row of the stretch is in registers ...
-    __syncthreads();                // ... in all waves, before any of them is overwritten
+#pragma unroll
+    for (int j = 0; j < kMoveRows; ++j) {
+      const int dst = first + j * kStep + (tid >> 3);
+      from[j] = src[j] != dst ? row_of(src[j]) : kNone;  // tokens in front of the first gap stay where they are
+      to[j] = src[j] != dst ? row_of(dst) : kNone;
+    }
+  };
+  find_rows(p.sink);
+  for (int first = p.sink; first < p.budget; first += kStep * kMoveRows) {
+    u32x4 v[kMoveRows];
+    char* dst[kMoveRows];
+#pragma unroll
+    for (int j = 0; j < kMoveRows; ++j) {
+      const bool move = from[j] != kNone && to[j] != kNone;
+      dst[j] = move ? address(to[j]) : nullptr;
+      if (move) v[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(address(from[j])));
+    }
+    find_rows(first + kStep * kMoveRows);  // of the next stretch, while these rows arrive
+    __builtin_amdgcn_s_waitcnt(0);         // every row of the stretch is in registers ...
+    __syncthreads();                       // ... in all waves, before any of them is overwritten
 #pragma unroll
     for (int j = 0; j < kMoveRows; ++j)
-      if (to[j]) *reinterpret_cast<u32x4*>(to[j]) = v[j];
+      if (dst[j]) *reinterpret_cast<u32x4*>(dst[j]) = v[j];
   }
 }
 
@@ -223,6 +241,8 @@ static int evict_tokens_impl(const char* fn, void* kv_cache, const float* scores
   if (score_stride < 1 || score_blocks < 0 || (!slot_ids && score_blocks < batch) || (slot_ids && score_blocks < 1))
     return fail(KIN_ERR_BAD_SHAPE, "%s: scores of %d rows of %d entries for batch=%d", fn, score_blocks, score_stride, batch);
   if (!aligned16(kv_cache)) return fail(KIN_ERR_MISALIGNED, "%s: kv_cache must be 16-byte aligned", fn);
+  if (num_pages > 0xffffffffLL / page_size - 1)
+    return fail(KIN_ERR_UNSUPPORTED, "%s: num_pages=%lld is too many", fn, (long long)num_pages);
   const int parts = head_dim * 2 / 128;
   if ((int64_t)batch * num_kv_heads * 2 * parts > 0x7fffffffLL)
     return fail(KIN_ERR_UNSUPPORTED, "%s: batch*num_kv_heads is too large", fn);
