@@ -6,7 +6,7 @@
 // then one ordered pass that writes the list of kept tokens and moves their scores.  evict_move_kernel moves the
 // K and V rows along that list, in place: a kept token never moves to a higher place, so a workgroup
 // that reads a stretch of the list before it writes it, and takes the stretches in order, overwrites only
-// rows that it has read.  K and V, and every 128 bytes of a row, move independently and get workgroups of their own.
+// rows that it has read.  K and V, and the parts of a row, move independently and get workgroups of their own.
 #include "kin_common.h"
 
 namespace kin {
@@ -16,7 +16,9 @@ constexpr int kEvictPer = 8;        // tokens per lane and step of the ordered p
 constexpr int kDigitBits = 11;      // of the radix search: sign, exponent and two bits of the fraction come first, so that scores of
 constexpr int kDigits = 1 << kDigitBits;  // one size do not all count in one place (LDS atomics on one address queue up)
 constexpr int kMoveThreads = 1024;
-constexpr int kMoveRows = 8;        // rows per lane in flight: a stretch is 1024 rows, 128 KiB of registers
+constexpr int kMoveRows = 8;        // rows per lane in flight: a stretch is 128 KiB of registers
+constexpr int kFewKeys = 256;       // so many keys that share the cut's first digits are ranked against one another at once
+constexpr int kKeepKeys = 16;       // keys a lane keeps in registers for the search (16384 tokens; the others are read again)
 
 struct EvictParams {
   uint16_t* kv;
@@ -56,9 +58,11 @@ __device__ __forceinline__ EvictSeq evict_seq(const EvictParams& p, int b) {
 }
 
 __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams p) {
-  __shared__ uint32_t hist[kDigits];
+  __shared__ uint32_t hist[4][kDigits];  // four lanes of a wave that meet the same digit count it in four places
   __shared__ uint32_t pick[2];   // digit that holds the cut, keys above it
   __shared__ uint32_t wave_above[kEvictThreads / 64];
+  __shared__ __attribute__((aligned(16))) uint32_t few[kFewKeys];
+  __shared__ uint32_t num_few, num_keys;
   __shared__ int2 wave_sum[kEvictThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = blockIdx.x / p.hkv, h = blockIdx.x - b * p.hkv;
@@ -84,19 +88,35 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams
   const int c0 = p.sink, c1 = n - p.local;
   uint32_t cut = 0, above = 0;
   if (m > 0) {
+    uint32_t key[kKeepKeys];
+    const int mine = max((c1 - c0 - tid + kEvictThreads - 1) / kEvictThreads, 0);  // this lane's tokens: c0 + tid + j * 1024
+#pragma unroll
+    for (int j = 0; j < kKeepKeys; ++j) key[j] = j < mine ? score_key(src[c0 + tid + j * kEvictThreads]) : 0;
+    auto for_keys = [&](auto f) {
+#pragma unroll
+      for (int j = 0; j < kKeepKeys; ++j)
+        if (j < mine) f(key[j]);
+      for (int j0 = kKeepKeys; j0 < mine; j0 += 8) {
+        uint32_t k[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) k[j] = j0 + j < mine ? score_key(src[c0 + tid + (j0 + j) * kEvictThreads]) : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j0 + j < mine) f(k[j]);
+      }
+    };
     for (int top = 32; top > 0; top -= kDigitBits) {  // bits below `top` are still open
       const int shift = max(top - kDigitBits, 0);
-      for (int d = tid; d < kDigits; d += kEvictThreads) hist[d] = 0;
+      for (int d = tid; d < 4 * kDigits; d += kEvictThreads) (&hist[0][0])[d] = 0;
       __syncthreads();
-#pragma unroll 8
-      for (int i = c0 + tid; i < c1; i += kEvictThreads) {
-        const uint32_t k = score_key(src[i]);
-        if (top == 32 || (k >> top) == (cut >> top)) atomicAdd(&hist[(k >> shift) & ((1u << (top - shift)) - 1)], 1u);
-      }
+      for_keys([&](uint32_t k) {
+        if (top == 32 || (k >> top) == (cut >> top)) atomicAdd(&hist[lane & 3][(k >> shift) & ((1u << (top - shift)) - 1)], 1u);
+      });
       __syncthreads();
       // thread t holds the digits kDigits - 1 - 2t and the one below: how many keys lie above them?
       const int d0 = kDigits - 1 - 2 * tid;
-      const uint32_t h0 = hist[d0], h1 = hist[d0 - 1];
+      const uint32_t h0 = hist[0][d0] + hist[1][d0] + hist[2][d0] + hist[3][d0];
+      const uint32_t h1 = hist[0][d0 - 1] + hist[1][d0 - 1] + hist[2][d0 - 1] + hist[3][d0 - 1];
       const uint32_t incl = wave_inclusive_sum(h0 + h1);
       if (lane == 63) wave_above[wave] = incl;
       __syncthreads();
@@ -105,13 +125,45 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams
       if (before < (uint32_t)m && before + h0 >= (uint32_t)m) {
         pick[0] = d0;
         pick[1] = before;
+        num_keys = h0;
       } else if (before + h0 < (uint32_t)m && before + h0 + h1 >= (uint32_t)m) {
         pick[0] = d0 - 1;
         pick[1] = before + h0;
+        num_keys = h1;
       }
+      if (tid == 0) num_few = 0;
+      if (tid < kFewKeys) few[tid] = 0;
       __syncthreads();
       cut |= pick[0] << shift;
       above = pick[1];
+      if (num_keys > kFewKeys || shift == 0) continue;
+      // Few keys share these digits: collect them (in any order) and rank each against the others.
+      for_keys([&](uint32_t k) {
+        if ((k >> shift) == (cut >> shift)) {
+          const uint32_t at = atomicAdd(&num_few, 1u);
+          if (at < kFewKeys) few[at] = k;
+        }
+      });
+      __syncthreads();
+      const uint32_t total = num_keys;
+      if (tid < (int)total) {
+        const uint32_t k = few[tid];
+        uint32_t over = 0, same = 0;
+#pragma unroll 4
+        for (uint32_t i = 0; i < total; i += 4) {  // zeros behind the last one: no score has key 0
+          const uint4 f = *reinterpret_cast<const uint4*>(few + i);
+          over += (f.x > k) + (f.y > k) + (f.z > k) + (f.w > k);
+          same += (f.x == k) + (f.y == k) + (f.z == k) + (f.w == k);
+        }
+        if (above + over < (uint32_t)m && above + over + same >= (uint32_t)m) {  // lanes with this very key write the same
+          pick[0] = k;
+          pick[1] = above + over;
+        }
+      }
+      __syncthreads();
+      cut = pick[0];
+      above = pick[1];
+      break;
     }
   }
   const int ties = m - (int)above;  // tokens with the cut score itself that stay, from the lowest index on
@@ -165,21 +217,23 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams
   for (int i = p.budget + tid; i < n; i += kEvictThreads) dst[i] = 0.f;
 }
 
-// blockIdx.x: 128-byte part of the row, K or V, head, sequence (part fastest).
+// A workgroup moves LPR * 16 bytes of every row of one (sequence, KV head, plane); the parts of a row are neighbours on one
+// XCD (workgroups go to the 8 XCDs in turn), whose L2 joins their accesses into whole lines.
+template <int LPR>
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p, int parts, int row_bytes) {
   const int tid = threadIdx.x;
-  int x = blockIdx.x;
-  const int part = x % parts;
-  x /= parts;
-  const int plane = x & 1;
-  x >>= 1;
-  const int h = x % p.hkv, b = x / p.hkv;
+  const int xcd = blockIdx.x % kNumXcds, rest = blockIdx.x / kNumXcds;
+  const int part = rest % parts;
+  const int64_t list = (int64_t)(rest / parts) * kNumXcds + xcd;  // plane fastest
+  if (list >= (int64_t)p.batch * p.hkv * 2) return;
+  const int plane = (int)(list & 1);
+  const int h = (int)((list >> 1) % p.hkv), b = (int)((list >> 1) / p.hkv);
   const EvictSeq sq = evict_seq(p, b);
   if (sq.blk < 0 || sq.len > p.stride || sq.len <= p.budget) return;
   const int32_t* kept = p.kept + ((int64_t)b * p.hkv + h) * p.budget;
   const int64_t page_bytes = 2ll * p.page_size * row_bytes;
   char* base = reinterpret_cast<char*>(p.kv) + (int64_t)plane * p.page_size * row_bytes + (int64_t)h * (row_bytes / p.hkv) +
-               part * 128 + (tid & 7) * 16;
+               (part * LPR + tid % LPR) * 16;
   // Row of the cache that holds a token (page * page_size + slot); none: its page is outside the cache.
   constexpr uint32_t kNone = 0xffffffffu;
   auto row_of = [&](int token) -> uint32_t {
@@ -190,18 +244,18 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p,
   auto address = [&](uint32_t row) -> char* {
     return base + (int64_t)(row >> p.page_shift) * page_bytes + (int64_t)(row & (p.page_size - 1)) * row_bytes;
   };
-  constexpr int kStep = kMoveThreads / 8;
+  constexpr int kStep = kMoveThreads / LPR;
   uint32_t from[kMoveRows], to[kMoveRows];
   auto find_rows = [&](int first) {
     int src[kMoveRows];
 #pragma unroll
     for (int j = 0; j < kMoveRows; ++j) {
-      const int dst = first + j * kStep + (tid >> 3);
+      const int dst = first + j * kStep + tid / LPR;
       src[j] = dst < p.budget ? kept[dst] : dst;
     }
 #pragma unroll
     for (int j = 0; j < kMoveRows; ++j) {
-      const int dst = first + j * kStep + (tid >> 3);
+      const int dst = first + j * kStep + tid / LPR;
       from[j] = src[j] != dst ? row_of(src[j]) : kNone;  // tokens in front of the first gap stay where they are
       to[j] = src[j] != dst ? row_of(dst) : kNone;
     }
@@ -243,8 +297,13 @@ static int evict_tokens_impl(const char* fn, void* kv_cache, const float* scores
   if (!aligned16(kv_cache)) return fail(KIN_ERR_MISALIGNED, "%s: kv_cache must be 16-byte aligned", fn);
   if (num_pages > 0xffffffffLL / page_size - 1)
     return fail(KIN_ERR_UNSUPPORTED, "%s: num_pages=%lld is too many", fn, (long long)num_pages);
-  const int parts = head_dim * 2 / 128;
-  if ((int64_t)batch * num_kv_heads * 2 * parts > 0x7fffffffLL)
+  // Bytes of a row per workgroup: whole lines of 128 if that makes a workgroup for every CU, else 64, else 32 (4 x 16384 to
+  // 4096 tokens of 8 heads, 128 / 64 bytes: 75 / 67 us; one such sequence, 128 / 64 / 32 bytes: 86 / 75 / 70 us).
+  const int64_t lists = ((int64_t)batch * num_kv_heads * 2 + kNumXcds - 1) / kNumXcds * kNumXcds;
+  int part_bytes = 128;
+  while (part_bytes > 32 && lists * (head_dim * 2 / part_bytes) < kNumCus) part_bytes /= 2;
+  const int parts = head_dim * 2 / part_bytes;
+  if (lists * parts > 0x7fffffffLL)
     return fail(KIN_ERR_UNSUPPORTED, "%s: batch*num_kv_heads is too large", fn);
   if (batch == 0) return KIN_OK;
   EvictParams p;
@@ -271,7 +330,11 @@ static int evict_tokens_impl(const char* fn, void* kv_cache, const float* scores
   hipStream_t s = static_cast<hipStream_t>(stream);
   evict_select_kernel<<<(unsigned)(batch * num_kv_heads), kEvictThreads, 0, s>>>(p);
   if (int st = check_hip(hipGetLastError(), "evict_select_kernel launch")) return st;
-  evict_move_kernel<<<(unsigned)(batch * num_kv_heads * 2 * parts), kMoveThreads, 0, s>>>(p, parts, num_kv_heads * head_dim * 2);
+  const unsigned grid = (unsigned)(lists * parts);
+  const int row_bytes = num_kv_heads * head_dim * 2;
+  if (part_bytes == 128) evict_move_kernel<8><<<grid, kMoveThreads, 0, s>>>(p, parts, row_bytes);
+  else if (part_bytes == 64) evict_move_kernel<4><<<grid, kMoveThreads, 0, s>>>(p, parts, row_bytes);
+  else evict_move_kernel<2><<<grid, kMoveThreads, 0, s>>>(p, parts, row_bytes);
   return check_hip(hipGetLastError(), "evict_move_kernel launch");
 }
 
