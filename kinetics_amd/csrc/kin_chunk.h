@@ -85,41 +85,57 @@ __device__ __forceinline__ bool row_sees(const RowSpan& r, int first, int slot) 
   return ((slot <= r.hi) & (slot >= r.lo)) | ((slot < r.prefix) & (slot >= first));
 }
 
-// tanh to about 3 units in the last place.  Below 3/4 x P(x^2) with P of degree 5 (least largest relative error on
-// that range, 3e-8 by its coefficients, 1.6e-7 with the fp32 roundings); beyond, 1 - 2 / (exp(2x) + 1), which no longer cancels.
-constexpr float kTanhSmall = 0.75f;
-__device__ __forceinline__ float tanh_small(float x) {
-  const float t = x * x;
+// tanh to about 3 units in the last place: x P(x^2) with the P of least largest relative error, of degree 3 below 1/4 (3e-9 by
+// its coefficients) and 5 below 3/4 (3e-8; 1.6e-7 with the fp32 roundings); beyond, 1 - 2 / (exp(2x) + 1), which no longer cancels.
+constexpr float kTanhTiny = 0.25f, kTanhSmall = 0.75f;
+__device__ __forceinline__ float tanh_over_x_tiny(float t) {
+  float y = fmaf(t, -0.051327724009752274f, 0.13323132693767548f);
+  y = fmaf(t, y, -0.3333320617675781f);
+  return fmaf(t, y, 1.0f);
+}
+__device__ __forceinline__ float tanh_over_x_small(float t) {
   float y = fmaf(t, -0.004716257564723492f, 0.01958290860056877f);
   y = fmaf(t, y, -0.05334443226456642f);
   y = fmaf(t, y, 0.1332540661096573f);
   y = fmaf(t, y, -0.33332958817481995f);
-  return x * fmaf(t, y, 1.0f);
+  return fmaf(t, y, 1.0f);
 }
 __device__ __forceinline__ float tanh_large(float x) {
   const float e = fast_exp2(fabsf(x) * (2.0f * kLog2e));
   return copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f), x);
 }
 
-// 16 raw products q.k of a lane as scores in log2 units, capped (without the distance bias).  Scores far below the
-// cap, which is what a cap is for, take the short form: 8 instead of about 24 issue slots each, chosen per block.
-__device__ __forceinline__ void cap_scores(const ChunkParams& p, floatx16& s) {
+// 16 raw products q.k of a lane as scores in log2 units, capped (without the distance bias), each minus z(e).  With x = score / cap
+// the capped score is (score) * (tanh(x) / x).  Scores far below the cap, which is what a cap is for, take the
+// short forms: 7 or 9 instead of about 24 issue slots each, chosen per block.
+template <typename Minus>
+__device__ __forceinline__ void cap_scores(const ChunkParams& p, floatx16& s, Minus z) {
   if (p.cap_log2 == 0.f) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] *= p.scale_log2;
+    for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], p.scale_log2, -z(e));
     return;
   }
   float top = 0.f;
 #pragma unroll
   for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(s[e]));
-  if (!__ballot(!(top * p.cap_in < kTanhSmall))) {
+  top *= p.cap_in;
+  if (!__ballot(!(top < kTanhTiny))) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) s[e] = p.cap_log2 * tanh_small(s[e] * p.cap_in);
+    for (int e = 0; e < 16; ++e) {
+      const float x = s[e] * p.cap_in;
+      s[e] = fmaf(s[e] * p.scale_log2, tanh_over_x_tiny(x * x), -z(e));
+    }
+  } else if (!__ballot(!(top < kTanhSmall))) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float x = s[e] * p.cap_in;
+      s[e] = fmaf(s[e] * p.scale_log2, tanh_over_x_small(x * x), -z(e));
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const float x = s[e] * p.cap_in;
-      s[e] = p.cap_log2 * (fabsf(x) < kTanhSmall ? tanh_small(x) : tanh_large(x));
+      s[e] = (fabsf(x) < kTanhSmall ? s[e] * p.scale_log2 * tanh_over_x_small(x * x) : p.cap_log2 * tanh_large(x)) - z(e);
     }
   }
 }

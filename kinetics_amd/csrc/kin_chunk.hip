@@ -147,7 +147,7 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
   after_k();
   if constexpr (EXTRA) {
 #pragma unroll
-    for (int t = 0; t < NSUB; ++t) cap_scores(p, s[t]);
+    for (int t = 0; t < NSUB; ++t) cap_scores(p, s[t], [](int) { return 0.f; });
     if (p.slopes) {
       const int pos = w.span.hi;  // the row's own token slot
 #pragma unroll

@@ -13,7 +13,6 @@
 namespace kin {
 
 constexpr int kMassKeys = 128;  // tokens of a workgroup
-constexpr int kMassRows = 64;   // rows of a staged tile (one per lane of a wave)
 
 struct MassParams {
   ChunkParams c;
@@ -24,17 +23,20 @@ struct MassParams {
   int key_tiles;            // workgroups per (sequence, KV head)
 };
 
-template <int HD, bool F16, bool EXTRA>
-__global__ __launch_bounds__(256, 2) void attention_mass_kernel(MassParams mp) {
+template <int HD, bool F16, bool EXTRA, int RW>
+__global__ __launch_bounds__(256 * RW, 2 * RW) void attention_mass_kernel(MassParams mp) {
   constexpr int kRowB = HD * 2;
+  constexpr int kMassRows = 64 * RW;  // rows of a staged tile
   constexpr int kStageB = kMassRows * kRowB;
-  constexpr int CPR = HD / 8, kLoads = kMassRows * CPR / 256;  // LDS-direct loads per wave and stage
+  constexpr int CPR = HD / 8, kLoads = 64 * CPR / 256;  // LDS-direct loads per wave and stage
   __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kStageB];
   __shared__ __attribute__((aligned(16))) float lse_sh[2][kMassRows], slope_sh[2][kMassRows];
   __shared__ __attribute__((aligned(16))) int hi_sh[2][kMassRows];
+  __shared__ float sum_sh[RW][kMassKeys];
   const ChunkParams& p = mp.c;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kw = wave & 3, rw = wave >> 2;  // which 32 tokens, and which share of the rows, the wave takes
   const int h = blockIdx.x % p.hkv;
   const int rest = blockIdx.x / p.hkv;
   const int b = rest / mp.key_tiles;
@@ -50,7 +52,7 @@ __global__ __launch_bounds__(256, 2) void attention_mass_kernel(MassParams mp) {
 
   for (int tile = rest % mp.key_tiles; tile * kMassKeys < end; tile += mp.key_tiles) {
     const int wg_slot0 = tile * kMassKeys;
-    const int slot0 = wg_slot0 + wave * 32;  // first token slot of the wave
+    const int slot0 = wg_slot0 + kw * 32;  // first token slot of the wave
     const int slot = slot0 + col;
     // this lane's key: chunk 2k + half of its row for step k
     uint4 key[HD / 16];
@@ -96,30 +98,30 @@ __global__ __launch_bounds__(256, 2) void attention_mass_kernel(MassParams mp) {
         lds_load_16<false>(rs, at + (wave * kLoads + j) * 1024, r0 + rr < last ? o : 0x7fff0000);
       }
     };
-    // its rows' log-sum-exp (log2), token slots and slopes: one row per thread of the first wave
+    // its rows' log-sum-exp (log2), token slots and slopes: one row per thread of the first waves
     float z = 0.f, sl = 0.f;
     int hi = 0;
     auto fetch_row = [&](int st) {
       const int r0 = first + st * kMassRows, i0s = r0 / p.group;
       int di, g;
-      split(r0 - i0s * p.group + lane, di, g);
+      split(r0 - i0s * p.group + tid, di, g);
       const int i = i0s + di;
-      const bool valid = r0 + lane < last;
+      const bool valid = r0 + tid < last;
       z = valid ? mp.lse[(int64_t)(sq.e0 + i) * p.hq + h * p.group + g] * kLog2e : INFINITY;
       if (z == kNegInf) z = INFINITY;  // a row that saw nothing gives nothing
       hi = base + i + off;
       if constexpr (EXTRA) sl = (p.slopes && valid) ? p.slopes[h * p.group + g] * kLog2e : 0.f;
     };
     auto put_row = [&](int st) {
-      lse_sh[st & 1][lane] = z;
-      hi_sh[st & 1][lane] = hi;
-      if constexpr (EXTRA) slope_sh[st & 1][lane] = sl;
+      lse_sh[st & 1][tid] = z;
+      hi_sh[st & 1][tid] = hi;
+      if constexpr (EXTRA) slope_sh[st & 1][tid] = sl;
     };
 
     float sum = 0.f;
     if (n_stages > 0) {
       stage_rows(0);
-      if (wave == 0) {
+      if (tid < kMassRows) {
         fetch_row(0);
         put_row(0);
       }
@@ -130,11 +132,12 @@ __global__ __launch_bounds__(256, 2) void attention_mass_kernel(MassParams mp) {
       const bool more = st + 1 < n_stages;
       if (more) {
         stage_rows(st + 1);
-        if (wave == 0) fetch_row(st + 1);
+        if (tid < kMassRows) fetch_row(st + 1);
       }
       const unsigned char* qs = lds + (st & 1) * kStageB;
 #pragma unroll
-      for (int t = 0; t < kMassRows / 32; ++t) {
+      for (int t2 = 0; t2 < 2; ++t2) {
+        const int t = t2 * RW + rw;
         const int r0 = first + st * kMassRows + t * 32;
         const int pos0 = base + r0 / p.group, pos1 = base + min(r0 + 31, last - 1) / p.group;
         if (r0 >= last || slot0 >= end) break;
@@ -152,14 +155,16 @@ __global__ __launch_bounds__(256, 2) void attention_mass_kernel(MassParams mp) {
         const float* zs = lse_sh[st & 1] + t * 32;
         const int* hs = hi_sh[st & 1] + t * 32;
         if constexpr (EXTRA) {
-          cap_scores(p, s);
+          cap_scores(p, s, [&](int e) { return zs[acc_row(e, half)]; });
           if (p.slopes) {
             const float* ss = slope_sh[st & 1] + t * 32;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = fmaf(-ss[acc_row(e, half)], (float)abs(hs[acc_row(e, half)] - slot), s[e]);
           }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] = fmaf(s[e], p.scale_log2, -zs[acc_row(e, half)]);
         }
-        const float c = EXTRA ? 1.f : p.scale_log2;
         if (!seen) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -170,21 +175,32 @@ __global__ __launch_bounds__(256, 2) void attention_mass_kernel(MassParams mp) {
         }
         float part = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) part += fast_exp2(fmaf(s[e], c, -zs[acc_row(e, half)]));
+        for (int e = 0; e < 16; ++e) part += fast_exp2(s[e]);
         sum += part;
       }
-      if (more && wave == 0) put_row(st + 1);
+      if (more && tid < kMassRows) put_row(st + 1);
     }
-    __syncthreads();  // the staging area is free for the next tile of keys
     sum += other_half(sum);
-    if (half == 0 && slot >= off && slot < end) dst[slot - off] += sum;
+    __syncthreads();  // the staging area is free for the next tile of keys
+    if constexpr (RW > 1) {
+      if (half == 0) sum_sh[rw][kw * 32 + col] = sum;
+      __syncthreads();
+      if (rw == 0)
+        for (int x = 1; x < RW; ++x) sum += sum_sh[x][kw * 32 + col];
+    }
+    if (rw == 0 && half == 0 && slot >= off && slot < end) dst[slot - off] += sum;
   }
 }
 
+template <int HD, bool F16, bool EXTRA>
+static void launch_mass(const MassParams& mp, unsigned grid, bool many_rows, hipStream_t s) {
+  if (many_rows) attention_mass_kernel<HD, F16, EXTRA, 2><<<grid, 512, 0, s>>>(mp);
+  else attention_mass_kernel<HD, F16, EXTRA, 1><<<grid, 256, 0, s>>>(mp);
+}
 template <int HD, bool F16>
-static void launch_mass(const MassParams& mp, unsigned grid, bool extra, hipStream_t s) {
-  if (extra) attention_mass_kernel<HD, F16, true><<<grid, 256, 0, s>>>(mp);
-  else attention_mass_kernel<HD, F16, false><<<grid, 256, 0, s>>>(mp);
+static void launch_mass(const MassParams& mp, unsigned grid, bool extra, bool many_rows, hipStream_t s) {
+  if (extra) launch_mass<HD, F16, true>(mp, grid, many_rows, s);
+  else launch_mass<HD, F16, false>(mp, grid, many_rows, s);
 }
 
 static int attention_mass_impl(const char* fn, bool f16, const void* q, const void* kv_cache, const float* lse, float* scores,
@@ -213,13 +229,14 @@ static int attention_mass_impl(const char* fn, bool f16, const void* q, const vo
   const int64_t grid = (int64_t)batch * num_kv_heads * mp.key_tiles;
   if (grid > 0x7fffffffLL) return fail(KIN_ERR_UNSUPPORTED, "%s: batch*num_kv_heads*max_pages_per_seq is too large", fn);
   const bool extra = slopes != nullptr || softcap > 0.f;
+  const bool many_rows = nnz * mp.c.group > 64 * (int64_t)batch;  // on average more than a stage of the small form
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == kHeadDimSmall) {
-    if (f16) launch_mass<kHeadDimSmall, true>(mp, (unsigned)grid, extra, s);
-    else launch_mass<kHeadDimSmall, false>(mp, (unsigned)grid, extra, s);
+    if (f16) launch_mass<kHeadDimSmall, true>(mp, (unsigned)grid, extra, many_rows, s);
+    else launch_mass<kHeadDimSmall, false>(mp, (unsigned)grid, extra, many_rows, s);
   } else {
-    if (f16) launch_mass<kHeadDim, true>(mp, (unsigned)grid, extra, s);
-    else launch_mass<kHeadDim, false>(mp, (unsigned)grid, extra, s);
+    if (f16) launch_mass<kHeadDim, true>(mp, (unsigned)grid, extra, many_rows, s);
+    else launch_mass<kHeadDim, false>(mp, (unsigned)grid, extra, many_rows, s);
   }
   return check_hip(hipGetLastError(), "attention_mass_kernel launch");
 }
