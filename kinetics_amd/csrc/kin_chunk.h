@@ -38,6 +38,7 @@ struct ChunkParams {
   int first_page_offset, window;
   float scale_log2;               // sm_scale * log2 e
   float cap_in, cap_log2;         // sm_scale / cap, cap * log2 e (cap_log2 == 0: no cap)
+  float cap_tiny[4];              // scale_log2 * kTanhTinyPoly[i] * cap_in^(2i): a small capped score straight from the raw product
 };
 
 // One sequence of the batch as the kernels see it; positions are token indices.
@@ -88,11 +89,7 @@ __device__ __forceinline__ bool row_sees(const RowSpan& r, int first, int slot) 
 // tanh to about 3 units in the last place: x P(x^2) with the P of least largest relative error, of degree 3 below 1/4 (3e-9 by
 // its coefficients) and 5 below 3/4 (3e-8; 1.6e-7 with the fp32 roundings); beyond, 1 - 2 / (exp(2x) + 1), which no longer cancels.
 constexpr float kTanhTiny = 0.25f, kTanhSmall = 0.75f;
-__device__ __forceinline__ float tanh_over_x_tiny(float t) {
-  float y = fmaf(t, -0.051327724009752274f, 0.13323132693767548f);
-  y = fmaf(t, y, -0.3333320617675781f);
-  return fmaf(t, y, 1.0f);
-}
+constexpr double kTanhTinyPoly[4] = {1.0, -0.3333320617675781, 0.13323132693767548, -0.051327724009752274};
 __device__ __forceinline__ float tanh_over_x_small(float t) {
   float y = fmaf(t, -0.004716257564723492f, 0.01958290860056877f);
   y = fmaf(t, y, -0.05334443226456642f);
@@ -107,8 +104,9 @@ __device__ __forceinline__ float tanh_large(float x) {
 
 // 16 raw products q.k of a lane as scores in log2 units, capped (without the distance bias), each minus z(e).  With x = score / cap
 // the capped score is (score) * (tanh(x) / x).  Scores far below the cap, which is what a cap is for, take the
-// short forms: 7 or 9 instead of about 24 issue slots each, chosen per block.
-template <typename Minus>
+// short forms: 5 (READY: coefficients made for this scale, in four more scalar registers; the attention kernel has none left and is
+// 8 % faster with 7 slots and literals) or 9 instead of about 24 issue slots each, chosen per block.
+template <bool READY, typename Minus>
 __device__ __forceinline__ void cap_scores(const ChunkParams& p, floatx16& s, Minus z) {
   if (p.cap_log2 == 0.f) {
 #pragma unroll
@@ -122,8 +120,15 @@ __device__ __forceinline__ void cap_scores(const ChunkParams& p, floatx16& s, Mi
   if (!__ballot(!(top < kTanhTiny))) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const float x = s[e] * p.cap_in;
-      s[e] = fmaf(s[e] * p.scale_log2, tanh_over_x_tiny(x * x), -z(e));
+      if constexpr (READY) {
+        const float t = s[e] * s[e];
+        const float y = fmaf(t, fmaf(t, fmaf(t, p.cap_tiny[3], p.cap_tiny[2]), p.cap_tiny[1]), p.cap_tiny[0]);
+        s[e] = fmaf(s[e], y, -z(e));
+      } else {
+        const float x = s[e] * p.cap_in, t = x * x;
+        const float y = fmaf(t, fmaf(t, fmaf(t, (float)kTanhTinyPoly[3], (float)kTanhTinyPoly[2]), (float)kTanhTinyPoly[1]), 1.f);
+        s[e] = fmaf(s[e] * p.scale_log2, y, -z(e));
+      }
     }
   } else if (!__ballot(!(top < kTanhSmall))) {
 #pragma unroll

@@ -147,7 +147,7 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
   after_k();
   if constexpr (EXTRA) {
 #pragma unroll
-    for (int t = 0; t < NSUB; ++t) cap_scores(p, s[t], [](int) { return 0.f; });
+    for (int t = 0; t < NSUB; ++t) cap_scores<false>(p, s[t], [](int) { return 0.f; });
     if (p.slopes) {
       const int pos = w.span.hi;  // the row's own token slot
 #pragma unroll
@@ -671,6 +671,8 @@ void fill_chunk_params(ChunkParams& p, const void* q, const void* kv_cache, cons
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
   p.cap_in = softcap > 0.f ? scale / softcap : 0.f;
   p.cap_log2 = softcap > 0.f ? (float)((double)softcap * 1.4426950408889634) : 0.f;
+  double power = (double)scale * 1.4426950408889634;
+  for (int i = 0; i < 4; ++i, power *= (double)p.cap_in * p.cap_in) p.cap_tiny[i] = (float)(power * kTanhTinyPoly[i]);
 }
 
 // Row tiles of the launch, and the spans into which the keys are cut: enough for two workgroups per CU, none of

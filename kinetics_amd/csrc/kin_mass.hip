@@ -155,7 +155,7 @@ __global__ __launch_bounds__(256 * RW, 2 * RW) void attention_mass_kernel(MassPa
         const float* zs = lse_sh[st & 1] + t * 32;
         const int* hs = hi_sh[st & 1] + t * 32;
         if constexpr (EXTRA) {
-          cap_scores(p, s, [&](int e) { return zs[acc_row(e, half)]; });
+          cap_scores<true>(p, s, [&](int e) { return zs[acc_row(e, half)]; });
           if (p.slopes) {
             const float* ss = slope_sh[st & 1] + t * 32;
 #pragma unroll
