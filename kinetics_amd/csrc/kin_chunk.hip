@@ -31,8 +31,10 @@ struct ChunkAttnParams {
   float* lse;      // [nnz, hq] or null
   float* ws_o;     // [splits, nnz * hq, D] fp32, splits > 1 only
   float* ws_lse;   // [splits, nnz * hq] (log2 domain)
+  int32_t* ws_count;  // [nnz * hq]: spans of this row's keys
   int slots;       // row tiles over all sequences, some of them empty
-  int num_splits;
+  int num_splits;  // most spans of one row tile's keys (the launch's second dimension)
+  int span_narrow, span_wide;  // tiles of 64 keys in a span, for row tiles of up to 32 rows and for larger ones
 };
 
 typedef short shortx4 __attribute__((ext_vector_type(4)));
@@ -306,8 +308,11 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
   const int t_hi = pos1 >= 0 ? (pos1 + off) / kChunkKeys + 1 : 0;
   const int n_tiles = n_prefix + max(t_hi - t_lo, 0);
   auto tile_at = [&](int it) { return it < n_prefix ? it : it - n_prefix + t_lo; };
-  const int per_split = (n_tiles + ap.num_splits - 1) / ap.num_splits;
-  const int it0 = min(split * per_split, n_tiles), it1 = min(n_tiles, it0 + per_split);
+  // Spans: a tile with few keys has fewer than the launch provides for, often one, and writes its result itself.
+  const int per_span = max(narrow ? ap.span_narrow : ap.span_wide, (n_tiles + ap.num_splits - 1) / ap.num_splits);
+  const int spans = max((n_tiles + per_span - 1) / per_span, 1);
+  if (split >= spans) return;
+  const int it0 = split * per_span, it1 = min(n_tiles, it0 + per_span);
 
   // Rows: in the narrow form every wave holds all of them.
   const int row = (narrow ? 0 : wave * 32) + (lane & 31);
@@ -455,7 +460,8 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
       const float lse2 = none ? kNegInf : mm + __log2f(den);
       const int i = (r0 + r) / p.group, g = (r0 + r) - i * p.group;
       const int64_t hq = (int64_t)(sq.e0 + i) * p.hq + h * p.group + g;
-      if (ap.num_splits == 1) {
+      if (d == 0 && split == 0 && ap.num_splits > 1) ap.ws_count[hq] = spans;
+      if (spans == 1) {
         uint2 y;
         y.x = pack2<F16>(acc.x * inv, acc.y * inv);
         y.y = pack2<F16>(acc.z * inv, acc.w * inv);
@@ -540,7 +546,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
       for (int e = 0; e < 16; e += 4) {
         const int d = t * 32 + acc_row(e, half);
         const floatx4 x = {w.o[t][e] * inv, w.o[t][e + 1] * inv, w.o[t][e + 2] * inv, w.o[t][e + 3] * inv};
-        if (ap.num_splits == 1) {
+        if (spans == 1) {
           uint2 y;
           y.x = pack2<F16>(x[0], x[1]);
           y.y = pack2<F16>(x[2], x[3]);
@@ -550,14 +556,15 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
         }
       }
     if (half == 0) {
-      if (ap.num_splits > 1) ap.ws_lse[at] = lse2;
+      if (spans > 1) ap.ws_lse[at] = lse2;
       else if (ap.lse) ap.lse[hq] = lse2 * kLn2;
+      if (split == 0 && ap.num_splits > 1) ap.ws_count[hq] = spans;
     }
   }
 }
 
 // Joins the spans of the keys: HD / 4 lanes per (row, query head), GROUPS of them sharing its spans (few rows have many spans, and
-// reading those one after the other is all latency: 16 spans of 32 rows 7.3 us with one group).
+// reading those one after the other is all latency: 16 spans of 32 rows 7.3 us with one group, 3.0 us with eight).
 // Rows that belong to no sequence are left alone.
 template <int HD, bool F16, int GROUPS>
 __global__ __launch_bounds__(256) void merge_chunk_kernel(ChunkAttnParams ap) {
@@ -569,14 +576,15 @@ __global__ __launch_bounds__(256) void merge_chunk_kernel(ChunkAttnParams ap) {
   const int64_t x = (int64_t)blockIdx.x * ROWS + r;
   const int64_t tok = x / ap.c.hq;
   const bool mine = x < total && tok >= ap.c.q_indptr[0] && tok < ap.c.q_indptr[ap.c.batch];
+  const int spans = mine ? ap.ws_count[x] : 0;
   float mm = kNegInf, den = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (mine) {
+  if (spans > 1) {
 #pragma unroll 8
-    for (int s = g; s < ap.num_splits; s += GROUPS) mm = fmaxf(mm, ap.ws_lse[s * total + x]);
+    for (int s = g; s < spans; s += GROUPS) mm = fmaxf(mm, ap.ws_lse[s * total + x]);
     const float safe = mm == kNegInf ? 0.f : mm;
 #pragma unroll 8
-    for (int s = g; s < ap.num_splits; s += GROUPS) {
+    for (int s = g; s < spans; s += GROUPS) {
       const float f = fast_exp2(ap.ws_lse[s * total + x] - safe);
       const float4 o = *reinterpret_cast<const float4*>(ap.ws_o + (s * total + x) * HD + d);
       den += f;
@@ -611,7 +619,7 @@ __global__ __launch_bounds__(256) void merge_chunk_kernel(ChunkAttnParams ap) {
       acc.w = fmaf(f, o.w, acc.w);
     }
   }
-  if (!mine) return;
+  if (spans <= 1) return;  // no row, or one whose workgroup wrote the result
   const bool none = mm == kNegInf && den == 0.f;
   const float inv = none ? 0.f : 1.f / den;
   uint2 y;
@@ -675,22 +683,43 @@ void fill_chunk_params(ChunkParams& p, const void* q, const void* kv_cache, cons
   for (int i = 0; i < 4; ++i, power *= (double)p.cap_in * p.cap_in) p.cap_tiny[i] = (float)(power * kTanhTinyPoly[i]);
 }
 
-// Row tiles of the launch, and the spans into which the keys are cut: enough for two workgroups per CU, none of
-// them below 4 tiles of 64 keys.
+// Row tiles of the launch, and the spans into which their keys are cut.
 static int64_t chunk_slots(int64_t nnz, int batch, int group) { return nnz * group / kChunkRows + batch; }
 
-static int chunk_auto_splits(int64_t nnz, int batch, int num_q_heads, int num_kv_heads, int max_pages_per_seq, int page_size) {
+// Few rows per sequence on average: mostly decode.
+static bool mostly_decode(int64_t nnz, int batch, int group) { return nnz * group <= (int64_t)kChunkRows * batch; }
+
+struct ChunkSpans {
+  int splits, narrow, wide;  // most spans of a row tile; tiles of 64 keys in a span
+};
+// Wide row tiles: enough spans for two workgroups per CU; more would only write more partial results.  Narrow ones (decode)
+// leave almost nothing behind, but their sequences' lengths differ: about four times as many spans even them out (60
+// sequences of 301..8201 tokens beside four prompts, 8 KV heads of 64: one span 150 us, 4 / 8 / 16 workgroups per CU 134 / 131 / 128).  No span below 4 tiles.
+static ChunkSpans chunk_spans(int64_t nnz, int batch, int num_q_heads, int num_kv_heads, int max_pages_per_seq, int page_size,
+                              int num_splits) {
+  const int64_t tiles = ((int64_t)max_pages_per_seq * page_size + kChunkKeys - 1) / kChunkKeys;
   const int64_t wgs = chunk_slots(nnz, batch, num_q_heads / num_kv_heads) * num_kv_heads;
-  if (wgs <= 0) return 1;
-  int64_t want = (2 * kNumCus) / wgs;
-  const int64_t cap = (int64_t)max_pages_per_seq * page_size / (4 * kChunkKeys);
-  if (want > cap) want = cap;
-  if (want > 64) want = 64;
-  return want < 1 ? 1 : (int)want;
+  auto span_of = [&](int64_t want, int64_t least) {
+    if (want > 64 && num_splits == 0) want = 64;
+    const int64_t span = (tiles + want - 1) / want;
+    return (int)(span > least ? span : least);
+  };
+  ChunkSpans s;
+  if (num_splits > 0) {
+    s.narrow = s.wide = span_of(num_splits, 1);
+    s.splits = num_splits;
+    return s;
+  }
+  const int64_t wide = wgs > 0 && 2 * kNumCus > wgs ? 2 * kNumCus / wgs : 1;
+  const bool decode = mostly_decode(nnz, batch, num_q_heads / num_kv_heads);
+  s.wide = span_of(wide, 4);
+  s.narrow = decode && wgs > 0 ? span_of((8 * kNumCus + wgs - 1) / wgs, 4) : s.wide;
+  s.splits = (int)((tiles + s.narrow - 1) / s.narrow);
+  return s;
 }
 
 static size_t chunk_workspace(int64_t nnz, int num_q_heads, int head_dim, int splits) {
-  return splits <= 1 ? 0 : (size_t)nnz * num_q_heads * splits * (head_dim + 1) * sizeof(float);
+  return splits <= 1 ? 0 : (size_t)nnz * num_q_heads * ((size_t)splits * (head_dim + 1) + 1) * sizeof(float);
 }
 
 template <int HD, bool F16>
@@ -699,7 +728,7 @@ static void launch_chunk(const ChunkAttnParams& ap, dim3 grid, bool extra, hipSt
   else chunk_attn_kernel<HD, F16, false><<<grid, 256, 0, stream>>>(ap);
   if (ap.num_splits > 1) {
     const int64_t rows = (int64_t)ap.c.nnz * ap.c.hq;
-    if (ap.num_splits > 4) {
+    if (rows < 4096) {
       merge_chunk_kernel<HD, F16, 1024 / HD><<<(unsigned)rows, 256, 0, stream>>>(ap);
     } else {
       const int per = 1024 / HD;
@@ -725,8 +754,10 @@ static int chunk_attention_impl(const char* fn, bool f16, const void* q, const v
   ChunkAttnParams ap;
   const int64_t slots = chunk_slots(nnz, batch, num_q_heads / num_kv_heads);
   if (slots * num_kv_heads > 0x7fffffffLL) return fail(KIN_ERR_UNSUPPORTED, "%s: too many row tiles", fn);
-  ap.num_splits = num_splits > 0 ? num_splits
-                                 : chunk_auto_splits(nnz, batch, num_q_heads, num_kv_heads, max_pages_per_seq, page_size);
+  const ChunkSpans spans = chunk_spans(nnz, batch, num_q_heads, num_kv_heads, max_pages_per_seq, page_size, num_splits);
+  ap.num_splits = spans.splits;
+  ap.span_narrow = spans.narrow;
+  ap.span_wide = spans.wide;
   if (ap.num_splits > 1) {
     const size_t need = chunk_workspace(nnz, num_q_heads, head_dim, ap.num_splits);
     if (!workspace || workspace_bytes < need)
@@ -740,6 +771,7 @@ static int chunk_attention_impl(const char* fn, bool f16, const void* q, const v
   ap.lse = lse;
   ap.ws_o = static_cast<float*>(workspace);
   ap.ws_lse = ap.num_splits > 1 ? ap.ws_o + (size_t)ap.num_splits * nnz * num_q_heads * head_dim : nullptr;
+  ap.ws_count = ap.num_splits > 1 ? reinterpret_cast<int32_t*>(ap.ws_lse + (size_t)ap.num_splits * nnz * num_q_heads) : nullptr;
   ap.slots = (int)slots;
   const dim3 grid((unsigned)(slots * num_kv_heads), (unsigned)ap.num_splits);
   const bool extra = slopes != nullptr || softcap > 0.f;
@@ -763,9 +795,8 @@ size_t kin_chunk_workspace_bytes(int64_t nnz, int batch, int num_q_heads, int nu
   if (nnz <= 0 || batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 || max_pages_per_seq <= 0 ||
       page_size <= 0 || head_dim <= 0)
     return 0;
-  const int splits = num_splits > 0 ? num_splits
-                                    : kin::chunk_auto_splits(nnz, batch, num_q_heads, num_kv_heads, max_pages_per_seq, page_size);
-  return kin::chunk_workspace(nnz, num_q_heads, head_dim, splits);
+  return kin::chunk_workspace(nnz, num_q_heads, head_dim,
+                              kin::chunk_spans(nnz, batch, num_q_heads, num_kv_heads, max_pages_per_seq, page_size, num_splits).splits);
 }
 
 int kin_paged_chunk_attention(const kin_bf16_t* q, const kin_bf16_t* kv_cache, const int32_t* q_indptr,
