@@ -42,7 +42,8 @@
  * config, benchmark/blocktopk_decoder.py:104); page_size 16, 32, 64 or 128
  * (the reference's --page_size, benchmark/blocktopk.py:13; the token-granular
  * policies: 16 only);
- * num_q_heads % num_kv_heads == 0 and group size num_q_heads/num_kv_heads <= 16.
+ * num_q_heads % num_kv_heads == 0 and group size num_q_heads/num_kv_heads <= 16
+ * (kin_attention_mass: 128; kin_paged_chunk_attention: any).
  * Where a comment below says "16" for a page it means page_size.
  */
 #ifndef KINETICS_AMD_H

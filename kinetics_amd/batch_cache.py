@@ -41,16 +41,12 @@ token set is then LiteSys' own, token for token.
 ``attn_layer_skip`` (default ``[0]``: layer 0 stays dense, sparsity_utils.py:211)
 is honoured.
 Prefill writes its rows and the mean keys of the pages it completes with the
-ragged append kernel; its attention is not the accelerated path and runs on
-PyTorch's scaled_dot_product_attention (LiteSys calls flashinfer there,
-batch_cache.py:112-145).
+ragged append kernel and attends to the slot's pages with the chunk attention
+kernel (LiteSys calls flashinfer there, batch_cache.py:112-145).
 """
 from __future__ import annotations
 
-import math
-
 import torch
-import torch.nn.functional as F
 
 from . import _lib, ops
 
@@ -279,7 +275,7 @@ class PagedBatchKVManager:
                                        first_page_offset=self.pad)
         return out
 
-    # ------------------------------------------------------------------ prefill (not the accelerated path)
+    # ------------------------------------------------------------------ prefill
     def prefill_or_append(self, query_states, key_states, value_states, layer_idx, batch_idx):
         """One request: write its K/V rows into the slot's pages and refresh the
         mean keys of the pages that are now full (one ragged append), then causal
@@ -305,18 +301,11 @@ class PagedBatchKVManager:
         idx = self.pool.slot_table[slot, :n_pages].contiguous()
         ptr = torch.tensor([0, n_pages], dtype=torch.int32, device=self.device)
         last = torch.tensor([total + pad - (n_pages - 1) * self.page], dtype=torch.int32, device=self.device)
+        rows = torch.tensor([0, seq_len], dtype=torch.int32, device=self.device)
         # rows to their page slots, mean keys of the pages that are now full
-        ops.append_paged_kv_ragged(key_states[0].transpose(0, 1).contiguous(), value_states[0].transpose(0, 1).contiguous(),
-                                   torch.tensor([0, seq_len], dtype=torch.int32, device=self.device),
+        ops.append_paged_kv_ragged(key_states[0].transpose(0, 1).contiguous(), value_states[0].transpose(0, 1).contiguous(), rows,
                                    self.kv_cache[layer_idx], self.kbar[layer_idx][slot:slot + 1], idx, ptr, last)
-        pages = self.kv_cache[layer_idx][idx.long()]                                           # [n_pages, 2, self.page, Hkv, D]
-        k_all = pages[:, 0].reshape(n_pages * self.page, Hkv, D)[pad:total + pad].transpose(0, 1)   # [Hkv, total, D]
-        v_all = pages[:, 1].reshape(n_pages * self.page, Hkv, D)[pad:total + pad].transpose(0, 1)
-        G = self.num_attention_heads // Hkv
-        q = query_states[0]                                                                    # [Hq, s, D]
-        pos_q = torch.arange(offset, total, device=self.device)[:, None]
-        mask = torch.arange(total, device=self.device)[None, :] <= pos_q                       # causal with history
-        o = F.scaled_dot_product_attention(q[None], k_all.repeat_interleave(G, dim=0)[None],
-                                           v_all.repeat_interleave(G, dim=0)[None], attn_mask=mask[None, None],
-                                           scale=1.0 / math.sqrt(D))[0]                       # [Hq, s, D]
-        return o.transpose(0, 1).reshape(bsz, seq_len, self.hidden_size)
+        # causal with the slot's history, straight from its pages
+        q = query_states[0].transpose(0, 1).contiguous()                                       # [s, Hq, D]
+        o = ops.paged_chunk_attention(q, self.kv_cache[layer_idx], rows, idx, ptr, last, n_pages, first_page_offset=pad)
+        return o.reshape(bsz, seq_len, self.hidden_size)

@@ -27,7 +27,7 @@ int check_hip(hipError_t e, const char* what) {
 }
 
 int check_common_dims(const char* fn, int batch, int num_q_heads, int num_kv_heads,
-                      int head_dim, int page_size, bool small_head_dim_built) {
+                      int head_dim, int page_size, bool small_head_dim_built, int max_group) {
   if (batch < 0) return fail(KIN_ERR_BAD_SHAPE, "%s: batch=%d is negative", fn, batch);
   if (num_kv_heads < 1) return fail(KIN_ERR_BAD_SHAPE, "%s: num_kv_heads=%d must be >= 1", fn, num_kv_heads);
   if (num_q_heads < 1 || num_q_heads % num_kv_heads != 0)
@@ -40,9 +40,9 @@ int check_common_dims(const char* fn, int batch, int num_q_heads, int num_kv_hea
                 small_head_dim_built ? "64 and " : "", kHeadDim);
   if (!supported_page_size(page_size))
     return fail(KIN_ERR_UNSUPPORTED, "%s: page_size=%d unsupported (kernels are built for 16, 32, 64 and 128)", fn, page_size);
-  if (num_q_heads / num_kv_heads > kMaxGroup)
+  if (num_q_heads / num_kv_heads > max_group)
     return fail(KIN_ERR_UNSUPPORTED, "%s: GQA group %d unsupported (max %d)", fn, num_q_heads / num_kv_heads,
-                kMaxGroup);
+                max_group);
   return KIN_OK;
 }
 

@@ -203,7 +203,7 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32);
 int check_chunk_args(const char* fn, const void* q, const void* kv_cache, const int32_t* q_indptr, const int32_t* page_indices,
                      const int32_t* page_indptr, const int32_t* last_page_len, int64_t nnz, int batch, int num_q_heads,
                      int num_kv_heads, int head_dim, int page_size, int64_t num_pages, int max_pages_per_seq,
-                     int first_page_offset, float sm_scale, float softcap, int window);
+                     int first_page_offset, float sm_scale, float softcap, int window, int max_group);
 void fill_chunk_params(ChunkParams& p, const void* q, const void* kv_cache, const int32_t* q_indptr, const int32_t* page_indices,
                        const int32_t* page_indptr, const int32_t* last_page_len, const float* slopes, const int32_t* prefix_lens,
                        int64_t nnz, int batch, int num_q_heads, int num_kv_heads, int head_dim, int page_size, int64_t num_pages,

@@ -634,10 +634,10 @@ __global__ __launch_bounds__(256) void merge_chunk_kernel(ChunkAttnParams ap) {
 int check_chunk_args(const char* fn, const void* q, const void* kv_cache, const int32_t* q_indptr, const int32_t* page_indices,
                      const int32_t* page_indptr, const int32_t* last_page_len, int64_t nnz, int batch, int num_q_heads,
                      int num_kv_heads, int head_dim, int page_size, int64_t num_pages, int max_pages_per_seq,
-                     int first_page_offset, float sm_scale, float softcap, int window) {
+                     int first_page_offset, float sm_scale, float softcap, int window, int max_group) {
   if (!q || !kv_cache || !q_indptr || !page_indices || !page_indptr || !last_page_len)
     return fail(KIN_ERR_NULL_POINTER, "%s: null pointer argument", fn);
-  if (int st = check_common_dims(fn, batch, num_q_heads, num_kv_heads, head_dim, page_size, true)) return st;
+  if (int st = check_common_dims(fn, batch, num_q_heads, num_kv_heads, head_dim, page_size, true, max_group)) return st;
   if (int st = check_first_page_offset(fn, first_page_offset, page_size)) return st;
   if (nnz < 0) return fail(KIN_ERR_BAD_SHAPE, "%s: nnz=%lld is negative", fn, (long long)nnz);
   if (nnz * num_q_heads > 0x7fffffffLL / 2) return fail(KIN_ERR_UNSUPPORTED, "%s: nnz*num_q_heads is too large", fn);
@@ -746,7 +746,7 @@ static int chunk_attention_impl(const char* fn, bool f16, const void* q, const v
   if (!out) return fail(KIN_ERR_NULL_POINTER, "%s: null pointer argument", fn);
   if (int st = check_chunk_args(fn, q, kv_cache, q_indptr, page_indices, page_indptr, last_page_len, nnz, batch, num_q_heads,
                                 num_kv_heads, head_dim, page_size, num_pages, max_pages_per_seq, first_page_offset, sm_scale,
-                                softcap, window))
+                                softcap, window, num_q_heads))  // rows are (token, head) pairs: any group
     return st;
   if (num_splits < 0 || num_splits > 1024) return fail(KIN_ERR_BAD_SHAPE, "%s: num_splits=%d must be in [0, 1024]", fn, num_splits);
   if (!aligned16(out)) return fail(KIN_ERR_MISALIGNED, "%s: out must be 16-byte aligned", fn);

@@ -60,8 +60,9 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Shape rules every entry point shares.  Returns KIN_OK or records an error.
 // small_head_dim_built: the entry point also has kernels for head_dim 64 (the page path has, the
 // token-granular policies and the layer's row kernels have not).
+// max_group: the largest number of query heads per KV head the entry point is built for.
 int check_common_dims(const char* fn, int batch, int num_q_heads, int num_kv_heads,
-                      int head_dim, int page_size, bool small_head_dim_built = false);
+                      int head_dim, int page_size, bool small_head_dim_built = false, int max_group = kMaxGroup);
 // Range rules for the always-attended parts of a page list.
 int check_fixed_pages(const char* fn, int sink_pages, int local_tokens);
 // first_page_offset: padding slots at the start of every sequence's first page.

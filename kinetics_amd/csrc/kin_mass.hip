@@ -13,6 +13,7 @@
 namespace kin {
 
 constexpr int kMassKeys = 128;  // tokens of a workgroup
+constexpr int kMassMaxGroup = 128;  // so that the short division of its rows is exact
 
 struct MassParams {
   ChunkParams c;
@@ -76,7 +77,7 @@ __global__ __launch_bounds__(256 * RW, 2 * RW) void attention_mass_kernel(MassPa
     const int first = i0 * p.group, n_stages = i1 > i0 ? ((i1 - i0) * p.group + kMassRows - 1) / kMassRows : 0;
     const int last = min(i1 * p.group, rows);  // one past the last row to count
 
-    // Rows of a stage as (token, head): x = the head of the stage's first row plus the row, below 2^16 / 16, so that
+    // Rows of a stage as (token, head): x = the head of the stage's first row plus the row, below group + 128, so that
     // x / group is a product and a shift.
     const uint32_t magic = 65536u / p.group + 1;
     auto split = [&](int x, int& q, int& g) {
@@ -212,7 +213,7 @@ static int attention_mass_impl(const char* fn, bool f16, const void* q, const vo
   if (!lse || !scores) return fail(KIN_ERR_NULL_POINTER, "%s: null pointer argument", fn);
   if (int st = check_chunk_args(fn, q, kv_cache, q_indptr, page_indices, page_indptr, last_page_len, nnz, batch, num_q_heads,
                                 num_kv_heads, head_dim, page_size, num_pages, max_pages_per_seq, first_page_offset, sm_scale,
-                                softcap, window))
+                                softcap, window, kMassMaxGroup))
     return st;
   if (score_stride < 1 || score_blocks < 0 || (!slot_ids && score_blocks < batch) || (slot_ids && score_blocks < 1))
     return fail(KIN_ERR_BAD_SHAPE, "%s: scores of %d rows of %d entries for batch=%d", fn, score_blocks, score_stride, batch);

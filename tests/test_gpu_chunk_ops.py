@@ -99,6 +99,45 @@ def test_chunk_attention_in_spans(ops, splits, window):
     assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("mods", [dict(), dict(window=700), dict(softcap=20.0, prefix_lens=True)], ids=["plain", "window", "cap-prefix"])
+def test_chunk_attention_decode_and_prompts_in_one_call(ops, mods):
+    """Long single-token rows are cut into more spans than the prompt's rows, which may have one."""
+    pb = R.problem(32, [5000, 3001, 900, 17, 4097], [1, 2, 100, 1, 8], 4, 1, 128, 16, "bf16", tail_rows=1)
+    mods = with_tensors(pb, mods)
+    assert ops.chunk_workspace_bytes(pb.q.shape[0], 5, 4, 1, pb.max_pages) > 0
+    out, lse = attend(ops, pb, **mods)
+    check_attention(pb, out, lse, **mods)
+    again, lse2 = attend(ops, pb, **mods)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("hq,hkv", [(24, 1), (64, 1), (66, 2), (128, 1)])
+def test_large_groups(ops, hq, hkv):
+    """More query heads per KV head than the decode kernels take: rows are (token, head) pairs."""
+    pb = R.problem(33, [150, 40], [7, 40], hq, hkv, 64, 16, "bf16", 3)
+    mods = with_tensors(pb, dict(slopes=True, window=60))
+    out, lse = attend(ops, pb, **mods)
+    check_attention(pb, out, lse, **mods)
+    sc = torch.zeros(2, hkv, 160, device=DEV)
+    want, tol = R.mass(pb, lse, sc, **mods)
+    ops.attention_mass(pb.q, pb.kv, lse, sc, pb.q_indptr, pb.ids, pb.ptr, pb.last, pb.max_pages, first_page_offset=3, **mods)
+    assert bool(((sc.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("cap", [0.5, 3.0, 1000.0])
+def test_caps_below_and_above_the_scores(ops, cap):
+    """Every form of the tanh: scores far below the cap, near it and far above it, within one block too."""
+    pb = R.problem(34, [300, 257], [64, 1], 4, 1, 128, 16, "bf16")
+    pb.q[::3] *= 0.02
+    pb.q[1::7] *= 8
+    out, lse = attend(ops, pb, softcap=cap)
+    check_attention(pb, out, lse, softcap=cap)
+    sc = torch.zeros(2, 1, 300, device=DEV)
+    want, tol = R.mass(pb, lse, sc, softcap=cap)
+    ops.attention_mass(pb.q, pb.kv, lse, sc, pb.q_indptr, pb.ids, pb.ptr, pb.last, pb.max_pages, softcap=cap)
+    assert bool(((sc.double() - want).abs() <= tol).all())
+
+
 def test_chunk_attention_more_rows_than_tokens(ops):
     """Rows in front of a sequence see nothing: zeros and -inf; a prefix does not change that."""
     pb = R.problem(5, [3, 0, 40], [9, 4, 41], 4, 1, 128, 16, "bf16")
@@ -462,6 +501,41 @@ def test_captured_replays_and_another_stream(ops):
         torch.cuda.synchronize()
         for a, b in zip(want, (out, lse, sc, kept, lens, pb.kv)):
             assert torch.equal(a, b)
+
+
+def test_two_streams_at_once(ops):
+    """Two chunks on two streams, each with its own workspace (allocated by the call), give what they give alone."""
+    a = R.problem(71, [3000], [2], 8, 2, 128, 16, "bf16")
+    b = R.problem(72, [2000, 100], [64, 100], 8, 2, 128, 16, "bf16")
+    want = [attend(ops, a), attend(ops, b)]
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        got = []
+        for s, pb in ((s1, a), (s2, b)):
+            with torch.cuda.stream(s):
+                got.append(attend(ops, pb))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+
+
+def test_opcheck(ops):
+    """Schemas, fake kernels and mutation annotations of the four operators under AOT dispatch."""
+    from torch.library import opcheck
+
+    pb = R.problem(73, [100, 40], [3, 1], 4, 2, 128, 16, "bf16")
+    table = (pb.q_indptr, pb.ids, pb.ptr, pb.last, pb.max_pages)
+    lse = torch.empty(pb.q.shape[:2], device=DEV)
+    k = torch.ops.kinetics
+    opcheck(k.paged_chunk_attention.default, (pb.q, pb.kv, *table), dict(lse=lse, window=30))
+    ops.paged_chunk_attention(pb.q, pb.kv, *table, lse=lse)
+    opcheck(k.attention_mass.default, (pb.q, pb.kv, lse, torch.rand(2, 2, 128, device=DEV), *table))
+    opcheck(k.evict_tokens.default, (pb.kv, torch.rand(2, 2, 128, device=DEV), pb.ids, pb.ptr, pb.last, 64))
+    freq, axis = ops.rope_table(128, device=DEV)
+    w = torch.ones(128, dtype=torch.bfloat16, device=DEV)
+    opcheck(k.qkv_norm_rope_split.default, (torch.randn(5, 6 * 128, device=DEV).bfloat16(), w, w, 1e-6, i32([0, 5, 2, 9, 1]), freq, axis, 4, 1))
+    opcheck(k.qkv_norm_rope_split.default, (torch.randn(5, 6 * 128, device=DEV).bfloat16(), None, None, 1e-6, i32([0, 5, 2, 9, 1]), freq, axis, 4, 1))
 
 
 def test_the_run_of_them(ops):
