@@ -30,10 +30,18 @@ __global__ __launch_bounds__(256 * RW, 2 * RW) void attention_mass_kernel(MassPa
   constexpr int kMassRows = 64 * RW;  // rows of a staged tile
   constexpr int kStageB = kMassRows * kRowB;
   constexpr int CPR = HD / 8, kLoads = 64 * CPR / 256;  // LDS-direct loads per wave and stage
-  __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kStageB];
-  __shared__ __attribute__((aligned(16))) float lse_sh[2][kMassRows], slope_sh[2][kMassRows];
-  __shared__ __attribute__((aligned(16))) int hi_sh[2][kMassRows];
-  __shared__ float sum_sh[RW][kMassKeys];
+  struct Shared {  // the stages first: LDS-direct loads reach 64 KiB
+    unsigned char lds[2 * kStageB];
+    float lse[2][kMassRows], slope[2][kMassRows];
+    int hi[2][kMassRows];
+    float sum[RW][kMassKeys];
+  };
+  __shared__ __attribute__((aligned(16))) Shared sh;
+  unsigned char* lds = sh.lds;
+  auto& lse_sh = sh.lse;
+  auto& slope_sh = sh.slope;
+  auto& hi_sh = sh.hi;
+  auto& sum_sh = sh.sum;
   const ChunkParams& p = mp.c;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
