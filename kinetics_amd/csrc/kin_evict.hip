@@ -121,7 +121,8 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams
       if (lane == 63) wave_above[wave] = incl;
       __syncthreads();
       uint32_t before = above + incl - h0 - h1;
-      for (int w = 0; w < wave; ++w) before += wave_above[w];
+#pragma unroll
+      for (int w = 0; w < kEvictThreads / 64; ++w) before += w < wave ? wave_above[w] : 0;
       if (before < (uint32_t)m && before + h0 >= (uint32_t)m) {
         pick[0] = d0;
         pick[1] = before;
@@ -188,6 +189,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams
     if (lane == 0) wave_sum[wave] = make_int2(ns, nt);
     __syncthreads();
     int s = sure0, t = tie0;
+#pragma unroll
     for (int w = 0; w < kEvictThreads / 64; ++w) {
       const int2 v = wave_sum[w];
       if (w < wave) {
