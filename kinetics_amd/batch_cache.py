@@ -40,6 +40,15 @@ skip the padding slots
 token set is then LiteSys' own, token for token.
 ``attn_layer_skip`` (default ``[0]``: layer 0 stays dense, sparsity_utils.py:211)
 is honoured.
+A dense manager can instead bound what it keeps: with ``kv_budget=N`` every layer
+adds up, per KV head, the attention weight each cached token receives, and a
+sequence that has outgrown N tokens is cut back to N -- its first
+``kv_budget_sink`` (4) tokens, its newest ``kv_budget_local`` (64) and the heaviest
+of the rest, each head its own -- after a prefill chunk, and in decoding every
+``kv_budget_slack`` (64) steps (counted on the host: a captured step does what it did
+when it was captured).  ``kv_offset`` then counts the tokens in the cache; the
+caller's position ids are its own.  A slot needs pages for N tokens plus the
+longest chunk or the slack.
 Prefill writes its rows and the mean keys of the pages it completes with the
 ragged append kernel and attends to the slot's pages with the chunk attention
 kernel (LiteSys calls flashinfer there, batch_cache.py:112-145).
@@ -119,6 +128,16 @@ class PagedBatchKVManager:
         self.local_tokens = int(kwargs["attn_local"]) if self.sparse else 1
         if self.sparse and not 1 <= self.local_tokens <= 1009:
             raise NotImplementedError("attn_local must be in [1, 1009]")
+        self.kv_budget = kwargs.get("kv_budget")
+        if self.kv_budget is not None:
+            if self.sparse or self.strided is not None or self.token_topk is not None:
+                raise NotImplementedError("kv_budget goes with dense decoding only")
+            self.kv_budget = int(self.kv_budget)
+            self.budget_sink, self.budget_local = int(kwargs.get("kv_budget_sink", 4)), int(kwargs.get("kv_budget_local", 64))
+            self.budget_slack = int(kwargs.get("kv_budget_slack", 64))
+            if min(self.budget_sink, self.budget_local) < 0 or self.kv_budget <= self.budget_sink + self.budget_local or self.budget_slack < 1:
+                raise ValueError(f"kv_budget={self.kv_budget} must exceed kv_budget_sink + kv_budget_local = "
+                                 f"{self.budget_sink + self.budget_local}, and kv_budget_slack must be at least 1")
         # padding slots in front of every sequence: LiteSys' 4 sink tokens end page 0, its blocks are pages 1, 2, ...
         self.pad = self.page - 4 if self.sparse else 0
 
@@ -136,6 +155,14 @@ class PagedBatchKVManager:
         # mean keys by SLOT; the kernels find a sequence's row block through slot_ids
         self.kbar = [torch.zeros(B, Hkv, P, D, dtype=dtype, device=dev) for _ in range(self.num_layers)]
         self.kv_offset = [torch.zeros(B, dtype=torch.int32, device=dev) for _ in range(self.num_layers)]
+        if self.kv_budget is not None:
+            # weight received so far, by slot; the entry of a token that is not there is 0
+            self.scores = [torch.zeros(B, Hkv, P * self.page, dtype=torch.float32, device=dev) for _ in range(self.num_layers)]
+            self._rows = torch.arange(B + 1, dtype=torch.int32, device=dev)    # q_indptr of one token per sequence
+            self._kept = torch.empty(B, Hkv, self.kv_budget, dtype=torch.int32, device=dev)
+            self._new_lens = torch.empty(B, dtype=torch.int32, device=dev)
+            self._lse = torch.empty(B, Hq, dtype=torch.float32, device=dev)
+            self._decode_steps = 0
         # Page-table metadata of the ACTIVE batch (sequence b of a launch = the b-th entry of batch_idx),
         # built on the device by the first layer of a decode step and reused by the other layers.
         self.page_indices = torch.zeros(self.num_pool_pages, dtype=torch.int32, device=dev)
@@ -193,6 +220,8 @@ class PagedBatchKVManager:
         written for it and its output was zero)."""
         for i in range(self.num_layers):
             self.kv_offset[i][batch_idx] = 0
+            if self.kv_budget is not None:
+                self.scores[i][batch_idx].zero_()
         self.pool.release(torch.tensor([int(batch_idx)], dtype=torch.int32, device=self.device))
         self._step_batch_idx = None
         self.pool.raise_on_overflow()
@@ -209,6 +238,8 @@ class PagedBatchKVManager:
         if fresh:
             n = batch_idx.numel()
             self._step_batch_idx = batch_idx
+            if self.kv_budget is not None:
+                self._decode_steps += 1
             self._slots32[:n].copy_(batch_idx, non_blocking=True)
             self._slots64[:n].copy_(batch_idx, non_blocking=True)
             self._step = (n, self._slots32[:n], self._slots64[:n], self._indptr[: n + 1], self._last[:n], self._one[:n])
@@ -270,10 +301,26 @@ class PagedBatchKVManager:
                 ops.block_score_topk(q, kbar, idx, indptr, last, self.block_topk, sel, cnt, sink_pages=self.sink_pages,
                                      local_tokens=self.local_tokens, workspace=self._ws, page_size=self.page, slot_ids=slots)
                 ops.sparse_paged_decode(q, kv, sel, cnt, last, out=out, workspace=self._ws, first_page_offset=self.pad)
-            else:
+            elif self.kv_budget is None:
                 ops.dense_paged_decode(q, kv, idx, indptr, last, self.pages_per_slot, out=out, workspace=self._ws,
                                        first_page_offset=self.pad)
+            else:
+                lse = self._lse[:n]
+                ops.dense_paged_decode(q, kv, idx, indptr, last, self.pages_per_slot, out=out, lse=lse, workspace=self._ws)
+                ops.attention_mass(q, kv, lse, self.scores[layer_idx], self._rows[: n + 1], idx, indptr, last, self.pages_per_slot,
+                                   slot_ids=slots)
+                if self._decode_steps % self.budget_slack == 0:    # every layer of this step
+                    _, lens = self._evict(layer_idx, idx, indptr, last, slots)
+                    offset = self.kv_offset[layer_idx]     # a sequence the pool could not serve (no pages) keeps its count
+                    offset.index_copy_(0, self._step[2], torch.where(lens > 0, lens, offset.index_select(0, self._step[2])))
         return out
+
+    def _evict(self, layer_idx, idx, indptr, last, slots):
+        """Cut the layer's sequences back to the budget (those within it stay as they are)."""
+        n = slots.numel()
+        return ops.evict_tokens(self.kv_cache[layer_idx], self.scores[layer_idx], idx, indptr, last, self.kv_budget,
+                                sink_tokens=self.budget_sink, local_tokens=self.budget_local, kept=self._kept[:n],
+                                new_lens=self._new_lens[:n], slot_ids=slots)
 
     # ------------------------------------------------------------------ prefill
     def prefill_or_append(self, query_states, key_states, value_states, layer_idx, batch_idx):
@@ -307,5 +354,12 @@ class PagedBatchKVManager:
                                    self.kv_cache[layer_idx], self.kbar[layer_idx][slot:slot + 1], idx, ptr, last)
         # causal with the slot's history, straight from its pages
         q = query_states[0].transpose(0, 1).contiguous()                                       # [s, Hq, D]
-        o = ops.paged_chunk_attention(q, self.kv_cache[layer_idx], rows, idx, ptr, last, n_pages, first_page_offset=pad)
+        lse = None if self.kv_budget is None else torch.empty(seq_len, self.num_attention_heads, device=self.device)
+        o = ops.paged_chunk_attention(q, self.kv_cache[layer_idx], rows, idx, ptr, last, n_pages, lse=lse, first_page_offset=pad)
+        if self.kv_budget is not None:
+            slots = torch.tensor([slot], dtype=torch.int32, device=self.device)
+            ops.attention_mass(q, self.kv_cache[layer_idx], lse, self.scores[layer_idx], rows, idx, ptr, last, n_pages, slot_ids=slots)
+            if total > self.kv_budget:
+                self._evict(layer_idx, idx, ptr, last, slots)
+                self.kv_offset[layer_idx][slot] = self.kv_budget
         return o.reshape(bsz, seq_len, self.hidden_size)
