@@ -614,3 +614,22 @@ def test_refusals(ops):
                  (qkv, w, w, 1e-6, i32([0, 1, 2]), freq, axis, 5, 1)):
         with pytest.raises(ValueError):
             ops.qkv_norm_rope_split(*args)
+
+
+@pytest.mark.parametrize("group", [1, 3, 4])
+@pytest.mark.parametrize("news", [1, 3, 50, 170])
+def test_infinite_keys_with_no_weight(ops, news, group):
+    """Keys whose scores are -inf for every row have weight 0, in tiles that are full of rows and in those that are not."""
+    pb = R.problem(91, [300, 200], [news, news], group, 1, 128, 16, "bf16")
+    pb.q[..., 0] = pb.q[..., 0].abs() + 0.25
+    for b, t in ((0, 5), (0, 140), (0, 299), (1, 40)):
+        page, slot = R.slot_of(pb, b, torch.tensor([t], device=DEV))
+        pb.kv[page, 0, slot, 0, 0] = -math.inf
+    out, lse = attend(ops, pb)
+    check_attention(pb, out, lse)
+    start = torch.rand(2, 1, 310, device=DEV)
+    sc = start.clone()
+    ops.attention_mass(pb.q, pb.kv, lse, sc, pb.q_indptr, pb.ids, pb.ptr, pb.last, pb.max_pages)
+    want, tol = R.mass(pb, lse, start)
+    assert bool(((sc.double() - want).abs() <= tol).all())
+    assert float(sc[0, 0, 5]) == float(start[0, 0, 5]) and float(sc[1, 0, 40]) == float(start[1, 0, 40])
