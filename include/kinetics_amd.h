@@ -731,6 +731,7 @@ int kin_blocktopk_decode_step_f16(const kin_f16_t* q, const kin_f16_t* k, const 
  *   s = softcap * tanh(s / softcap)        with softcap > 0
  *   s = s - slopes[g] * |p - j|            with slopes != NULL (fp32 [num_q_heads])
  * Distances count the tokens that are in the cache.
+ * (sm_scale * log2 e and sm_scale / softcap must be finite in fp32.)
  *
  * max_pages_per_seq: the longest page list, for planning only (a smaller number
  * costs time, not tokens).  Page ids outside [0, num_pages) are never

@@ -312,7 +312,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) 
   if (b < 0) return;
   const int rows = sq.n * p.group;   // int: nnz * group is checked on the host
   const int r0 = (slot - first_slot(p, sq.e0, b)) * kChunkRows;
-  if (r0 >= rows) return;
+  if (r0 < 0 || r0 >= rows) return;  // below 0: q_indptr does not ascend
   const int nrows = min(rows - r0, kChunkRows);
   const bool narrow = nrows <= 32;   // uniform
 
@@ -595,7 +595,7 @@ __global__ __launch_bounds__(256) void merge_chunk_kernel(ChunkAttnParams ap) {
   const int64_t x = (int64_t)blockIdx.x * ROWS + r;
   const int64_t tok = x / ap.c.hq;
   const bool mine = x < total && tok >= ap.c.q_indptr[0] && tok < ap.c.q_indptr[ap.c.batch];
-  const int spans = mine ? ap.ws_count[x] : 0;
+  const int spans = mine ? min(ap.ws_count[x], ap.num_splits) : 0;  // min: a row nobody counted (q_indptr does not ascend)
   float mm = kNegInf, den = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (spans > 1) {
@@ -667,6 +667,10 @@ int check_chunk_args(const char* fn, const void* q, const void* kv_cache, const 
   if (window < 0) return fail(KIN_ERR_BAD_SHAPE, "%s: window=%d is negative", fn, window);
   if (!(sm_scale >= 0.f) || std::isinf(sm_scale) || !(softcap >= 0.f) || std::isinf(softcap))
     return fail(KIN_ERR_BAD_SHAPE, "%s: sm_scale and softcap must be finite and not negative", fn);
+  // what the kernels multiply a raw product with
+  const float scale = sm_scale > 0.f ? sm_scale : 1.0f / sqrtf((float)head_dim);
+  if (std::isinf((float)((double)scale * 1.4426950408889634)) || (softcap > 0.f && std::isinf(scale / softcap)))
+    return fail(KIN_ERR_BAD_SHAPE, "%s: sm_scale=%g with softcap=%g is out of fp32's range", fn, sm_scale, softcap);
   if (!aligned16(q) || !aligned16(kv_cache))
     return fail(KIN_ERR_MISALIGNED, "%s: q and kv_cache must be 16-byte aligned", fn);
   return KIN_OK;
@@ -716,7 +720,8 @@ struct ChunkSpans {
 // sequences of 301..8201 tokens beside four prompts, 8 KV heads of 64: one span 150 us, 4 / 8 / 16 workgroups per CU 134 / 131 / 128).  No span below 4 tiles.
 static ChunkSpans chunk_spans(int64_t nnz, int batch, int num_q_heads, int num_kv_heads, int max_pages_per_seq, int page_size,
                               int num_splits) {
-  const int64_t tiles = ((int64_t)max_pages_per_seq * page_size + kChunkKeys - 1) / kChunkKeys;
+  int64_t tiles = ((int64_t)max_pages_per_seq * page_size + kChunkKeys - 1) / kChunkKeys;
+  if (tiles > 0x7fffffff) tiles = 0x7fffffff;  // spans are ints
   const int64_t wgs = chunk_slots(nnz, batch, num_q_heads / num_kv_heads) * num_kv_heads;
   auto span_of = [&](int64_t want, int64_t least) {
     if (want > 64 && num_splits == 0) want = 64;

@@ -147,3 +147,18 @@ def test_chunk_ops_have_fake_kernels_and_refuse_cpu_tensors():
         ops.evict_tokens(ckv, torch.zeros(2, 1, 64), ci, ci, ci[:2], 32)
     with pytest.raises(ValueError, match="GPU"):
         ops.qkv_norm_rope_split(torch.zeros(3, 768, dtype=torch.bfloat16), None, None, 1e-6, ci, *ops.rope_table(128, device="cpu"), 4, 1)
+
+
+def test_scales_out_of_range(lib):
+    """A scale or cap whose fp32 factors overflow would turn a score of 0 into NaN: refused."""
+    for bad in (dict(cap=1e-40), dict(scale=3e38), dict(scale=1e30, cap=1e-9)):
+        assert chunk(lib, **bad) == _lib.KIN_ERR_BAD_SHAPE, bad
+    assert mass(lib, cap=1e-40) == _lib.KIN_ERR_BAD_SHAPE
+    assert chunk(lib, cap=1e-30, nnz=0) == _lib.KIN_OK and chunk(lib, scale=1e30, nnz=0) == _lib.KIN_OK
+
+
+def test_chunk_workspace_bytes_of_the_longest_page_list(lib):
+    size = lib.kin_chunk_workspace_bytes
+    for ps in (16, 128):
+        assert size(1, 1, 4, 1, 2 ** 31 - 1, ps, 128, 0) == 4 * (64 * 129 + 1) * 4      # at most 64 spans
+        assert size(10 ** 6, 1, 4, 1, 2 ** 31 - 1, ps, 128, 0) == 0                       # one span of all of it

@@ -633,3 +633,11 @@ def test_infinite_keys_with_no_weight(ops, news, group):
     want, tol = R.mass(pb, lse, start)
     assert bool(((sc.double() - want).abs() <= tol).all())
     assert float(sc[0, 0, 5]) == float(start[0, 0, 5]) and float(sc[1, 0, 40]) == float(start[1, 0, 40])
+
+
+def test_q_indptr_that_does_not_ascend_stays_inside(ops):
+    """Out of contract, but no row is written that the table does not name."""
+    pb = R.problem(92, [40, 40], [3, 0], 4, 1, 128, 16, "bf16", tail_rows=197)
+    out = torch.full_like(pb.q, 5.0)
+    ops.paged_chunk_attention(pb.q, pb.kv, i32([200, 0, 3]), pb.ids, pb.ptr, pb.last, pb.max_pages, out=out)
+    assert bool((out[3:] == 5.0).all())
