@@ -23,6 +23,8 @@ namespace kin {
 
 constexpr int kChunkRows = 128;     // rows of a workgroup's tile
 constexpr int kChunkKeys = 64;      // keys of a staged tile
+// Workgroups on a CU: the registers of a wave's outputs allow 3 with heads of 64 and 2 with heads of 128.
+constexpr int chunk_wgs_per_cu(int head_dim) { return head_dim == kHeadDimSmall ? 3 : 2; }
 constexpr float kRescaleLog2 = 8.f; // the running maximum is only moved when a score passes it by 2^8
 
 struct ChunkAttnParams {
@@ -150,15 +152,26 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
   }
   if constexpr (!EXTRA) __builtin_amdgcn_s_setprio(0);
   after_k();
+  float bias = 0.f;  // what all of this lane's scores still lack
   if constexpr (EXTRA) {
 #pragma unroll
     for (int t = 0; t < NSUB; ++t) cap_scores<false>(p, s[t], [](int) { return 0.f; });
     if (p.slopes) {
-      const int pos = w.span.hi;  // the row's own token slot
+      // Register e is key slot0 + 4 half + k(e).  Where every key lies in front of the wave's rows, -slope |p - j| is a part that
+      // all of a lane's keys share and slope * k(e): one instruction per score.
+      const float dist = (float)(w.span.hi - slot0 - 4 * half);
+      if (!__ballot(w.span.hi >= 0 && w.span.hi < slot0 + 32 * NSUB - 1)) {
+        bias = -w.slope2 * dist;
 #pragma unroll
-      for (int t = 0; t < NSUB; ++t)
+        for (int t = 0; t < NSUB; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[t][e] = fmaf(-w.slope2, (float)abs(pos - (slot0 + t * 32 + acc_row(e, half))), s[t][e]);
+          for (int e = 0; e < 16; ++e) s[t][e] = fmaf(w.slope2, (float)(t * 32 + acc_row(e, 0)), s[t][e]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < NSUB; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[t][e] = fmaf(-w.slope2, fabsf(dist - (float)(t * 32 + acc_row(e, 0))), s[t][e]);
+      }
     }
   }
   if (masked) {
@@ -176,7 +189,7 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
   for (int t = 0; t < NSUB; ++t)
 #pragma unroll
     for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[t][e]);
-  mt = max_halves(mt);
+  mt = max_halves(EXTRA ? mt + bias : mt);
   // The reference maximum follows the scores only when they pass it by 2^8 (weights stay below 2^8, which both
   // element types and the fp32 sums hold without loss), so most blocks need no rescaling of O.
   const bool move = mt > w.m && !((mt - w.m) * c <= kRescaleLog2);
@@ -190,7 +203,7 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
 #pragma unroll
       for (int e = 0; e < 16; ++e) w.o[t][e] *= alpha;
   }
-  const float shift = w.m == kNegInf ? 0.f : w.m * c;
+  const float shift = (w.m == kNegInf ? 0.f : w.m * c) - (EXTRA ? bias : 0.f);
   // V^T: lane (16-lane group g = lane / 16 % 2, place q = lane % 16) asks for 4 columns of key row q / 4 and is handed
   // the 4 keys of column 16 g + q; two such reads make one operand (keys 4h.. and 8 + 4h..).
   const int q4 = (lane & 15) >> 2, cq = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), lo8 = (lane & 1) * 8;
@@ -292,7 +305,7 @@ __device__ __forceinline__ void put_specials(WaveRows<HD>& w) {
 }
 
 template <int HD, bool F16, bool EXTRA>
-__global__ __launch_bounds__(256, 2) void chunk_attn_kernel(ChunkAttnParams ap) {
+__global__ __launch_bounds__(256, chunk_wgs_per_cu(HD)) void chunk_attn_kernel(ChunkAttnParams ap) {
   constexpr int kRowB = HD * 2;
   constexpr int kUnitB = 16 * kRowB;             // 16 keys
   constexpr int kStageB = 2 * kChunkKeys * kRowB;  // 64 keys and their values
@@ -715,11 +728,12 @@ static bool mostly_decode(int64_t nnz, int batch, int group) { return nnz * grou
 struct ChunkSpans {
   int splits, narrow, wide;  // most spans of a row tile; tiles of 64 keys in a span
 };
-// Wide row tiles: enough spans for two workgroups per CU; more would only write more partial results.  Narrow ones (decode)
+// Wide row tiles: enough spans for every workgroup that fits on a CU (bias case of 211 row tiles, heads of 64: 2 / 3 / 4 per CU
+// 45.5 / 42.5 / 44.2 us); more would only write more partial results.  Narrow ones (decode)
 // leave almost nothing behind, but their sequences' lengths differ: about four times as many spans even them out (60
 // sequences of 301..8201 tokens beside four prompts, 8 KV heads of 64: one span 150 us, 4 / 8 / 16 workgroups per CU 134 / 131 / 128).  No span below 4 tiles.
 static ChunkSpans chunk_spans(int64_t nnz, int batch, int num_q_heads, int num_kv_heads, int max_pages_per_seq, int page_size,
-                              int num_splits) {
+                              int head_dim, int num_splits) {
   int64_t tiles = ((int64_t)max_pages_per_seq * page_size + kChunkKeys - 1) / kChunkKeys;
   if (tiles > 0x7fffffff) tiles = 0x7fffffff;  // spans are ints
   const int64_t wgs = chunk_slots(nnz, batch, num_q_heads / num_kv_heads) * num_kv_heads;
@@ -734,7 +748,8 @@ static ChunkSpans chunk_spans(int64_t nnz, int batch, int num_q_heads, int num_k
     s.splits = num_splits;
     return s;
   }
-  const int64_t wide = wgs > 0 && 2 * kNumCus > wgs ? 2 * kNumCus / wgs : 1;
+  const int64_t places = (int64_t)chunk_wgs_per_cu(head_dim) * kNumCus;
+  const int64_t wide = wgs > 0 && places > wgs ? places / wgs : 1;
   const bool decode = mostly_decode(nnz, batch, num_q_heads / num_kv_heads);
   s.wide = span_of(wide, 4);
   s.narrow = decode && wgs > 0 ? span_of((8 * kNumCus + wgs - 1) / wgs, 4) : s.wide;
@@ -778,7 +793,7 @@ static int chunk_attention_impl(const char* fn, bool f16, const void* q, const v
   ChunkAttnParams ap;
   const int64_t slots = chunk_slots(nnz, batch, num_q_heads / num_kv_heads);
   if (slots * num_kv_heads > 0x7fffffffLL) return fail(KIN_ERR_UNSUPPORTED, "%s: too many row tiles", fn);
-  const ChunkSpans spans = chunk_spans(nnz, batch, num_q_heads, num_kv_heads, max_pages_per_seq, page_size, num_splits);
+  const ChunkSpans spans = chunk_spans(nnz, batch, num_q_heads, num_kv_heads, max_pages_per_seq, page_size, head_dim, num_splits);
   ap.num_splits = spans.splits;
   ap.span_narrow = spans.narrow;
   ap.span_wide = spans.wide;
@@ -820,7 +835,7 @@ size_t kin_chunk_workspace_bytes(int64_t nnz, int batch, int num_q_heads, int nu
       page_size <= 0 || head_dim <= 0)
     return 0;
   return kin::chunk_workspace(nnz, num_q_heads, head_dim,
-                              kin::chunk_spans(nnz, batch, num_q_heads, num_kv_heads, max_pages_per_seq, page_size, num_splits).splits);
+                              kin::chunk_spans(nnz, batch, num_q_heads, num_kv_heads, max_pages_per_seq, page_size, head_dim, num_splits).splits);
 }
 
 int kin_paged_chunk_attention(const kin_bf16_t* q, const kin_bf16_t* kv_cache, const int32_t* q_indptr,

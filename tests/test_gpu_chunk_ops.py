@@ -641,3 +641,16 @@ def test_q_indptr_that_does_not_ascend_stays_inside(ops):
     out = torch.full_like(pb.q, 5.0)
     ops.paged_chunk_attention(pb.q, pb.kv, i32([200, 0, 3]), pb.ids, pb.ptr, pb.last, pb.max_pages, out=out)
     assert bool((out[3:] == 5.0).all())
+
+
+def test_thousands_of_sequences(ops):
+    """More sequences than the 64 x 64 that two steps of the search for a row tile's sequence cover."""
+    lens = [(7 * i) % 4 if i % 5 else 0 for i in range(4200)] + [33]
+    news = [min(n, (i // 3) % 3) for i, n in enumerate(lens)]
+    pb = R.problem(93, lens, news, 2, 1, 64, 16, "f16")
+    out, lse = attend(ops, pb)
+    check_attention(pb, out, lse)
+    sc = torch.zeros(len(lens), 1, 40, device=DEV)
+    ops.attention_mass(pb.q, pb.kv, lse, sc, pb.q_indptr, pb.ids, pb.ptr, pb.last, pb.max_pages)
+    want, tol = R.mass(pb, lse, torch.zeros_like(sc))
+    assert bool(((sc.double() - want).abs() <= tol).all())
