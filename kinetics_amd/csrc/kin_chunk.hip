@@ -17,6 +17,11 @@
 // four keys of one column.  P never leaves the registers.  P is rounded to the cache's element type
 // for the matrix unit (half a unit in the last place, as the result itself); the running sum and
 // maximum, and O, are fp32.
+//
+// What bounds it, measured in bf16 on MI355X: prompts the matrix unit (51 % busy), the LDS reads and the softmax together --
+// 8192 tokens from nothing, 32 heads on 8 of 128: 546 us, 1.0 PFLOP/s; 2048 behind 30720, 4 heads on 1: 155 us, 0.86 PFLOP/s.
+// Decode rows HBM: 60 single tokens of 301..8201 beside four prompts, 8 KV heads of 64: 129 us.  Few rows the chain of
+// dependent loads: 8 single tokens of 513..4097: 8 us and 4 for the join.
 #include "kin_chunk.h"
 
 namespace kin {

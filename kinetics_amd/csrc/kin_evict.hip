@@ -7,6 +7,8 @@
 // K and V rows along that list, in place: a kept token never moves to a higher place, so a workgroup
 // that reads a stretch of the list before it writes it, and takes the stretches in order, overwrites only
 // rows that it has read.  K and V, and the parts of a row, move independently and get workgroups of their own.
+// 4 sequences of 16384 to 4096 tokens, 8 heads of 128: search 23 us (32 lists, 32 workgroups: the LDS histogram and two ordered
+// steps of each), move 43 us (134 MB of rows of 256 bytes in random places, 3.1 TB/s).  96 of about 1100 to 1024: 10 and 12 us.
 #include "kin_common.h"
 
 namespace kin {

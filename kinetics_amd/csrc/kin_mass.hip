@@ -7,7 +7,9 @@
 // once and stay in registers as the matrix unit's operand, and the rows pass by, 64 at a time, through two
 // stages in LDS that all four waves read.  S = Q K^T on v_mfma_f32_32x32x16 leaves lane l the scores of ONE token (column l % 32) against
 // 16 rows, so the sum over rows is a sum over registers: no atomics, one owner per token, and the order of
-// the additions never changes.  One exponential per (row, token): with many rows that is what bounds it.
+// the additions never changes.  With many rows the vector unit bounds it, one exponential and seven slots per (row, token) with a
+// cap: 2048 rows of 8192 tokens, 32 heads on 8: 222 us.  With single tokens it is the reading of the keys: 256 sequences of
+// 1025..8193, 83 us, 3.7 TB/s.  (Rows straight from L2 instead of through LDS: 469 us for the first.)
 #include "kin_chunk.h"
 
 namespace kin {

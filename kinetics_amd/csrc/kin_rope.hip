@@ -2,7 +2,8 @@
 // (as kin_qkv_norm_split; optional), and rotary positions with one or several axes (text: one; images and
 // video: time, height, width).  Pair i of a head, its elements i and i + D/2, is turned by
 //     angle = position[axis[i]] * frequency[i].
-// HBM-bound: every row is read once and written once with 16-byte accesses.
+// HBM-bound: every row is read once and written once with 16-byte accesses (8191 tokens, 32 + 2 * 8 heads of 128, three axes:
+// 35 us, 5.8 TB/s; 4096 tokens of 4 + 2 heads: 6 us).
 //
 // Positions run to millions, where an fp32 angle has no digits left behind the full turns.  Frequencies are
 // therefore turns per position as 64-bit fractions: position times fraction, modulo 2^64, IS the angle
@@ -25,8 +26,8 @@ struct RopeParams {
   float eps;
 };
 
-// Sum of squares, scaling: one element at a time, fp32, like the norm of kin_qkv_norm_split but without its rounding
-// between norm and rotation.
+// 16-bit elements of a 16-byte chunk and back.  Norm and rotation are fp32 in between, with one rounding at the end
+// (kin_qkv_norm_split rounds after its norm).
 template <bool F16>
 __device__ __forceinline__ void unpack8(const u32x4& v, float (&x)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
