@@ -7,19 +7,22 @@
 // K and V rows along that list, in place: a kept token never moves to a higher place, so a workgroup
 // that reads a stretch of the list before it writes it, and takes the stretches in order, overwrites only
 // rows that it has read.  K and V, and the parts of a row, move independently and get workgroups of their own.
-// 4 sequences of 16384 to 4096 tokens, 8 heads of 128: search 23 us (32 lists, 32 workgroups: the LDS histogram and two ordered
-// steps of each), move 43 us (134 MB of rows of 256 bytes in random places, 3.1 TB/s).  96 of about 1100 to 1024: 10 and 12 us.
+// 4 sequences of 16384 to 4096 tokens, 8 heads of 128: search 19 us (32 lists, 32 workgroups: loads, an LDS histogram and two
+// ordered steps of each, one behind the other), move 38 us (134 MB of rows of 256 bytes in random places, 3.5 TB/s).  96 of about
+// 1100 to 1024: 11 and 12 us.  Loads under a condition are written with a clamped index: as branches, each one waited for the
+// one before it (search 23 us, move 43).
 #include "kin_common.h"
 
 namespace kin {
 
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictPer = 8;        // tokens per lane and step of the ordered pass
-constexpr int kDigitBits = 11;      // of the radix search: sign, exponent and two bits of the fraction come first, so that scores of
-constexpr int kDigits = 1 << kDigitBits;  // one size do not all count in one place (LDS atomics on one address queue up)
+constexpr int kDigitBits = 13;      // of the radix search: sign, exponent and four bits of the fraction come first, so that mostly
+constexpr int kDigits = 1 << kDigitBits;  // few keys share the cut's digit and LDS atomics, which queue up on one address, spread (11 bits: 37 us for equal scores; 24)
+constexpr int kDigitsPer = kDigits / kEvictThreads;
 constexpr int kMoveThreads = 1024;
 constexpr int kMoveRows = 8;        // rows per lane in flight: a stretch is 128 KiB of registers
-constexpr int kFewKeys = 256;       // so many keys that share the cut's first digits are ranked against one another at once
+constexpr int kFewKeys = kEvictThreads / 4;  // so many keys that share the cut's first digits are ranked against one another at once
 constexpr int kKeepKeys = 16;       // keys a lane keeps in registers for the search (16384 tokens; the others are read again)
 
 struct EvictParams {
@@ -60,7 +63,7 @@ __device__ __forceinline__ EvictSeq evict_seq(const EvictParams& p, int b) {
 }
 
 __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams p) {
-  __shared__ uint32_t hist[4][kDigits];  // four lanes of a wave that meet the same digit count it in four places
+  __shared__ __attribute__((aligned(16))) uint32_t hist[2][kDigits];  // even and odd lanes count in places of their own
   __shared__ uint32_t pick[2];   // digit that holds the cut, keys above it
   __shared__ uint32_t wave_above[kEvictThreads / 64];
   __shared__ __attribute__((aligned(16))) uint32_t few[kFewKeys];
@@ -86,14 +89,14 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams
       for (int i = tid; i < n; i += kEvictThreads) dst[i] = src[i];
     return;
   }
-  // The m-th largest key of the tokens sink .. n - local - 1, a digit at a time from the top (11, 11, 10 bits).
+  // The m-th largest key of the tokens sink .. n - local - 1, a digit at a time from the top (13, 13, 6 bits).
   const int c0 = p.sink, c1 = n - p.local;
   uint32_t cut = 0, above = 0;
   if (m > 0) {
     uint32_t key[kKeepKeys];
     const int mine = max((c1 - c0 - tid + kEvictThreads - 1) / kEvictThreads, 0);  // this lane's tokens: c0 + tid + j * 1024
 #pragma unroll
-    for (int j = 0; j < kKeepKeys; ++j) key[j] = j < mine ? score_key(src[c0 + tid + j * kEvictThreads]) : 0;
+    for (int j = 0; j < kKeepKeys; ++j) key[j] = score_key(src[min(c0 + tid + j * kEvictThreads, c1 - 1)]);  // min, not a branch: all loads at once
     auto for_keys = [&](auto f) {
 #pragma unroll
       for (int j = 0; j < kKeepKeys; ++j)
@@ -101,7 +104,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams
       for (int j0 = kKeepKeys; j0 < mine; j0 += 8) {
         uint32_t k[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) k[j] = j0 + j < mine ? score_key(src[c0 + tid + (j0 + j) * kEvictThreads]) : 0;
+        for (int j = 0; j < 8; ++j) k[j] = score_key(src[min(c0 + tid + (j0 + j) * kEvictThreads, c1 - 1)]);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (j0 + j < mine) f(k[j]);
@@ -109,30 +112,48 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams
     };
     for (int top = 32; top > 0; top -= kDigitBits) {  // bits below `top` are still open
       const int shift = max(top - kDigitBits, 0);
-      for (int d = tid; d < 4 * kDigits; d += kEvictThreads) (&hist[0][0])[d] = 0;
+      for (int d = tid * 4; d < 2 * kDigits; d += kEvictThreads * 4) *reinterpret_cast<uint4*>(&hist[0][0] + d) = uint4{0, 0, 0, 0};
       __syncthreads();
       for_keys([&](uint32_t k) {
-        if (top == 32 || (k >> top) == (cut >> top)) atomicAdd(&hist[lane & 3][(k >> shift) & ((1u << (top - shift)) - 1)], 1u);
+        if (top == 32 || (k >> top) == (cut >> top)) {
+          const uint32_t d = (k >> shift) & ((1u << (top - shift)) - 1);
+          const uint64_t here = __ballot(true);
+          if (__ballot(d == (uint32_t)__builtin_amdgcn_readfirstlane((int)d)) == here) {  // one digit for all: one of them counts
+            if (lane == __builtin_ctzll(here)) atomicAdd(&hist[0][d], (uint32_t)__popcll(here));
+          } else {
+            atomicAdd(&hist[lane & 1][d], 1u);
+          }
+        }
       });
       __syncthreads();
-      // thread t holds the digits kDigits - 1 - 2t and the one below: how many keys lie above them?
-      const int d0 = kDigits - 1 - 2 * tid;
-      const uint32_t h0 = hist[0][d0] + hist[1][d0] + hist[2][d0] + hist[3][d0];
-      const uint32_t h1 = hist[0][d0 - 1] + hist[1][d0 - 1] + hist[2][d0 - 1] + hist[3][d0 - 1];
-      const uint32_t incl = wave_inclusive_sum(h0 + h1);
+      // thread t holds 8 digits, from kDigits - 8t - 1 down: how many keys lie above them?
+      const int d0 = kDigits - kDigitsPer * (tid + 1);
+      uint32_t h[kDigitsPer], sum = 0;
+#pragma unroll
+      for (int i = 0; i < kDigitsPer; i += 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(&hist[0][d0 + i]), y = *reinterpret_cast<const uint4*>(&hist[1][d0 + i]);
+        h[i] = x.x + y.x;
+        h[i + 1] = x.y + y.y;
+        h[i + 2] = x.z + y.z;
+        h[i + 3] = x.w + y.w;
+        sum += h[i] + h[i + 1] + h[i + 2] + h[i + 3];
+      }
+      const uint32_t incl = wave_inclusive_sum(sum);
       if (lane == 63) wave_above[wave] = incl;
       __syncthreads();
-      uint32_t before = above + incl - h0 - h1;
+      uint32_t before = above + incl - sum;
 #pragma unroll
       for (int w = 0; w < kEvictThreads / 64; ++w) before += w < wave ? wave_above[w] : 0;
-      if (before < (uint32_t)m && before + h0 >= (uint32_t)m) {
-        pick[0] = d0;
-        pick[1] = before;
-        num_keys = h0;
-      } else if (before + h0 < (uint32_t)m && before + h0 + h1 >= (uint32_t)m) {
-        pick[0] = d0 - 1;
-        pick[1] = before + h0;
-        num_keys = h1;
+      if (before < (uint32_t)m && before + sum >= (uint32_t)m) {  // one thread: the cut is in its digits
+#pragma unroll
+        for (int i = kDigitsPer - 1; i >= 0; --i) {
+          if (before < (uint32_t)m && before + h[i] >= (uint32_t)m) {
+            pick[0] = d0 + i;
+            pick[1] = before;
+            num_keys = h[i];
+          }
+          before += h[i];
+        }
       }
       if (tid == 0) num_few = 0;
       if (tid < kFewKeys) few[tid] = 0;
@@ -148,20 +169,22 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams
         }
       });
       __syncthreads();
-      const uint32_t total = num_keys;
-      if (tid < (int)total) {
-        const uint32_t k = few[tid];
-        uint32_t over = 0, same = 0;
-#pragma unroll 4
-        for (uint32_t i = 0; i < total; i += 4) {  // zeros behind the last one: no score has key 0
-          const uint4 f = *reinterpret_cast<const uint4*>(few + i);
-          over += (f.x > k) + (f.y > k) + (f.z > k) + (f.w > k);
-          same += (f.x == k) + (f.y == k) + (f.z == k) + (f.w == k);
-        }
-        if (above + over < (uint32_t)m && above + over + same >= (uint32_t)m) {  // lanes with this very key write the same
-          pick[0] = k;
-          pick[1] = above + over;
-        }
+      // four threads to a key, each against a quarter of the others (zeros behind the last one: no score has key 0)
+      const uint32_t total = num_keys, k = few[tid / 4];
+      uint32_t over = 0, same = 0;
+#pragma unroll 2
+      for (uint32_t i = (tid & 3) * 4; i < total; i += 16) {
+        const uint4 f = *reinterpret_cast<const uint4*>(few + i);
+        over += (f.x > k) + (f.y > k) + (f.z > k) + (f.w > k);
+        same += (f.x == k) + (f.y == k) + (f.z == k) + (f.w == k);
+      }
+      over += __shfl_xor(over, 1);
+      same += __shfl_xor(same, 1);
+      over += __shfl_xor(over, 2);
+      same += __shfl_xor(same, 2);
+      if (k != 0 && above + over < (uint32_t)m && above + over + same >= (uint32_t)m) {  // threads with this very key write the same
+        pick[0] = k;
+        pick[1] = above + over;
       }
       __syncthreads();
       cut = pick[0];
@@ -178,9 +201,10 @@ __global__ __launch_bounds__(kEvictThreads) void evict_select_kernel(EvictParams
     int ns = 0, nt = 0;
     const int first = base + wave * 64 * kEvictPer + lane;
 #pragma unroll
+    for (int j = 0; j < kEvictPer; ++j) x[j] = src[min(first + j * 64, n - 1)];
+#pragma unroll
     for (int j = 0; j < kEvictPer; ++j) {
       const int i = first + j * 64;
-      x[j] = i < n ? src[i] : 0.f;
       const uint32_t k = score_key(x[j]);
       const bool mid = i >= c0 && i < c1;
       sure[j] = __ballot(i < n && (!mid || (m > 0 && k > cut)));
@@ -238,11 +262,10 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p,
   const int64_t page_bytes = 2ll * p.page_size * row_bytes;
   char* base = reinterpret_cast<char*>(p.kv) + (int64_t)plane * p.page_size * row_bytes + (int64_t)h * (row_bytes / p.hkv) +
                (part * LPR + tid % LPR) * 16;
-  // Row of the cache that holds a token (page * page_size + slot); none: its page is outside the cache.
+  // Row of the cache (page * page_size + slot) that holds a token on page `id`; none: the page is outside the cache.
   constexpr uint32_t kNone = 0xffffffffu;
-  auto row_of = [&](int token) -> uint32_t {
+  auto row_of = [&](int token, int id) -> uint32_t {
     const int at = token + p.first_page_offset;
-    const int id = sq.pages[at >> p.page_shift];
     return id >= 0 && (int64_t)id < p.num_pages ? ((uint32_t)id << p.page_shift) + (at & (p.page_size - 1)) : kNone;
   };
   auto address = [&](uint32_t row) -> char* {
@@ -251,17 +274,22 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p,
   constexpr int kStep = kMoveThreads / LPR;
   uint32_t from[kMoveRows], to[kMoveRows];
   auto find_rows = [&](int first) {
-    int src[kMoveRows];
+    // all loads of a kind at once, none behind a branch that would wait for it (tokens behind the budget: the last one's)
+    int src[kMoveRows], dst[kMoveRows], from_page[kMoveRows], to_page[kMoveRows];
 #pragma unroll
     for (int j = 0; j < kMoveRows; ++j) {
-      const int dst = first + j * kStep + tid / LPR;
-      src[j] = dst < p.budget ? kept[dst] : dst;
+      dst[j] = min(first + j * kStep + tid / LPR, p.budget - 1);
+      src[j] = kept[dst[j]];
+      to_page[j] = sq.pages[(dst[j] + p.first_page_offset) >> p.page_shift];
     }
 #pragma unroll
+    for (int j = 0; j < kMoveRows; ++j) from_page[j] = sq.pages[(src[j] + p.first_page_offset) >> p.page_shift];
+#pragma unroll
     for (int j = 0; j < kMoveRows; ++j) {
-      const int dst = first + j * kStep + tid / LPR;
-      from[j] = src[j] != dst ? row_of(src[j]) : kNone;  // tokens in front of the first gap stay where they are
-      to[j] = src[j] != dst ? row_of(dst) : kNone;
+      // tokens in front of the first gap stay where they are
+      const bool move = src[j] != dst[j] && first + j * kStep + tid / LPR < p.budget;
+      from[j] = move ? row_of(src[j], from_page[j]) : kNone;
+      to[j] = move ? row_of(dst[j], to_page[j]) : kNone;
     }
   };
   find_rows(p.sink);
@@ -274,7 +302,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictParams p,
       dst[j] = move ? address(to[j]) : nullptr;
       if (move) v[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(address(from[j])));
     }
-    find_rows(first + kStep * kMoveRows);  // of the next stretch, while these rows arrive
+    if (first + kStep * kMoveRows < p.budget) find_rows(first + kStep * kMoveRows);  // of the next stretch, while these rows arrive
     __builtin_amdgcn_s_waitcnt(0);         // every row of the stretch is in registers ...
     __syncthreads();                       // ... in all waves, before any of them is overwritten
 #pragma unroll
@@ -302,7 +330,8 @@ static int evict_tokens_impl(const char* fn, void* kv_cache, const float* scores
   if (num_pages > 0xffffffffLL / page_size - 1)
     return fail(KIN_ERR_UNSUPPORTED, "%s: num_pages=%lld is too many", fn, (long long)num_pages);
   // Bytes of a row per workgroup: whole lines of 128 if that makes a workgroup for every CU, else 64, else 32 (4 x 16384 to
-  // 4096 tokens of 8 heads, 128 / 64 bytes: 75 / 67 us; one such sequence, 128 / 64 / 32 bytes: 86 / 75 / 70 us).
+  // 4096 tokens of 8 heads, 128 / 64 / 32 bytes: 70 / 61 / 74 us; 96 of about 1100 to 1024, one head: 25 / 28 / 36 us; one
+  // sequence of 32768 to 4096: 72 / 62 / 56 us).
   const int64_t lists = ((int64_t)batch * num_kv_heads * 2 + kNumXcds - 1) / kNumXcds * kNumXcds;
   int part_bytes = 128;
   while (part_bytes > 32 && lists * (head_dim * 2 / part_bytes) < kNumCus) part_bytes /= 2;

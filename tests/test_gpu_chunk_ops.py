@@ -654,3 +654,16 @@ def test_thousands_of_sequences(ops):
     ops.attention_mass(pb.q, pb.kv, lse, sc, pb.q_indptr, pb.ids, pb.ptr, pb.last, pb.max_pages)
     want, tol = R.mass(pb, lse, torch.zeros_like(sc))
     assert bool(((sc.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("n,budget", [(20000, 5000), (17000, 16900), (700, 300)])
+def test_evict_tokens_whose_scores_differ_in_their_last_bits(ops, n, budget):
+    """Every digit of the search is needed, and more keys than it ranks at once share the upper ones."""
+    pb = R.problem(94, [n], [0], 1, 1, 64, 64, "bf16", 7)
+    g = torch.Generator().manual_seed(94)
+    for spread in (3000, 40):
+        sc = (1.0 + torch.randint(0, spread, (1, 1, n + 5), generator=g).double() * 2.0 ** -23).float().to(DEV)
+        kv, scores, kept, lens = R.evict(pb, sc, budget, 4, 100)
+        got, new = ops.evict_tokens(pb.kv, sc, pb.ids, pb.ptr, pb.last, budget, sink_tokens=4, local_tokens=100, first_page_offset=7)
+        assert torch.equal(got, kept) and torch.equal(new, lens) and torch.equal(sc, scores)
+        assert torch.equal(pb.kv.view(torch.int16), kv.view(torch.int16))
