@@ -44,10 +44,10 @@ A dense manager can instead bound what it keeps: with ``kv_budget=N`` every laye
 adds up, per KV head, the attention weight each cached token receives, and a
 sequence that has outgrown N tokens is cut back to N -- its first
 ``kv_budget_sink`` (4) tokens, its newest ``kv_budget_local`` (64) and the heaviest
-of the rest, each head its own -- after a prefill chunk, and in decoding every
-``kv_budget_slack`` (64) steps (counted on the host: a captured step does what it did
-when it was captured).  ``kv_offset`` then counts the tokens in the cache; the
-caller's position ids are its own.  A slot needs pages for N tokens plus the
+of the rest, each head its own -- after a prefill chunk, and in decoding when it
+has come to N + ``kv_budget_slack`` (64) tokens, which the device decides for every
+sequence in every step, captured ones included.  ``kv_offset`` then counts the tokens
+in the cache; the caller's position ids are its own.  A slot needs pages for N tokens plus the
 longest chunk or the slack.
 Prefill writes its rows and the mean keys of the pages it completes with the
 ragged append kernel and attends to the slot's pages with the chunk attention
@@ -162,7 +162,7 @@ class PagedBatchKVManager:
             self._kept = torch.empty(B, Hkv, self.kv_budget, dtype=torch.int32, device=dev)
             self._new_lens = torch.empty(B, dtype=torch.int32, device=dev)
             self._lse = torch.empty(B, Hq, dtype=torch.float32, device=dev)
-            self._decode_steps = 0
+            self._cut = None                 # of the active batch: (slots, -1 for a sequence that is not cut in this step; counts after it)
         # Page-table metadata of the ACTIVE batch (sequence b of a launch = the b-th entry of batch_idx),
         # built on the device by the first layer of a decode step and reused by the other layers.
         self.page_indices = torch.zeros(self.num_pool_pages, dtype=torch.int32, device=dev)
@@ -238,8 +238,6 @@ class PagedBatchKVManager:
         if fresh:
             n = batch_idx.numel()
             self._step_batch_idx = batch_idx
-            if self.kv_budget is not None:
-                self._decode_steps += 1
             self._slots32[:n].copy_(batch_idx, non_blocking=True)
             self._slots64[:n].copy_(batch_idx, non_blocking=True)
             self._step = (n, self._slots32[:n], self._slots64[:n], self._indptr[: n + 1], self._last[:n], self._one[:n])
@@ -251,6 +249,10 @@ class PagedBatchKVManager:
             # a slot that crossed a page boundary takes a page from the pool
             self.pool.reserve(lens, slots)
             self.pool.build_page_table(lens, self.page_indices, indptr, last, slots)
+            if self.kv_budget is not None:
+                # a sequence the pool could not serve (no pages) is not cut and keeps its count
+                cut = (lens >= self.kv_budget + self.budget_slack) & (indptr[1:] > indptr[:-1])
+                self._cut = torch.where(cut, slots, -1), torch.where(cut, self.kv_budget, lens)
         return n, slots, indptr, last
 
     def _advance(self, layer_idx):
@@ -294,7 +296,8 @@ class PagedBatchKVManager:
                     slot_lens=self.kv_offset[layer_idx])     # the kernel advances the slots' offsets itself
             plan(q, k, v, out)
         else:
-            self._advance(layer_idx)
+            if self.kv_budget is None:     # with a budget the counts after the step are known already
+                self._advance(layer_idx)
             ops.append_paged_kv(k, v, kv, kbar, idx, indptr, last, slot_ids=slots)
             if sparse:
                 sel, cnt = self._sel[:n], self._cnt[:n]
@@ -309,18 +312,17 @@ class PagedBatchKVManager:
                 ops.dense_paged_decode(q, kv, idx, indptr, last, self.pages_per_slot, out=out, lse=lse, workspace=self._ws)
                 ops.attention_mass(q, kv, lse, self.scores[layer_idx], self._rows[: n + 1], idx, indptr, last, self.pages_per_slot,
                                    slot_ids=slots)
-                if self._decode_steps % self.budget_slack == 0:    # every layer of this step
-                    _, lens = self._evict(layer_idx, idx, indptr, last, slots)
-                    offset = self.kv_offset[layer_idx]     # a sequence the pool could not serve (no pages) keeps its count
-                    offset.index_copy_(0, self._step[2], torch.where(lens > 0, lens, offset.index_select(0, self._step[2])))
+                cut_slots, counts = self._cut
+                self._evict(layer_idx, idx, indptr, last, cut_slots)
+                self.kv_offset[layer_idx].index_copy_(0, self._step[2], counts)
         return out
 
     def _evict(self, layer_idx, idx, indptr, last, slots):
-        """Cut the layer's sequences back to the budget (those within it stay as they are)."""
+        """Cut the layer's sequences back to the budget (those within it, and those with slot -1, stay as they are)."""
         n = slots.numel()
-        return ops.evict_tokens(self.kv_cache[layer_idx], self.scores[layer_idx], idx, indptr, last, self.kv_budget,
-                                sink_tokens=self.budget_sink, local_tokens=self.budget_local, kept=self._kept[:n],
-                                new_lens=self._new_lens[:n], slot_ids=slots)
+        ops.evict_tokens(self.kv_cache[layer_idx], self.scores[layer_idx], idx, indptr, last, self.kv_budget,
+                         sink_tokens=self.budget_sink, local_tokens=self.budget_local, kept=self._kept[:n],
+                         new_lens=self._new_lens[:n], slot_ids=slots)
 
     # ------------------------------------------------------------------ prefill
     def prefill_or_append(self, query_states, key_states, value_states, layer_idx, batch_idx):
