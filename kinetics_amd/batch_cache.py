@@ -143,6 +143,9 @@ class PagedBatchKVManager:
 
         B, Hq, Hkv, D = max_batch_size, self.num_attention_heads, self.num_key_value_heads, self.head_dim
         self.pages_per_slot = P = (max_seq_len + self.pad + self.page - 1) // self.page
+        if self.kv_budget is not None and self.kv_budget + self.budget_slack > P * self.page:
+            raise ValueError(f"kv_budget + kv_budget_slack = {self.kv_budget + self.budget_slack} tokens must fit a slot's {P} pages of "
+                             f"{self.page} (max_seq_len={max_seq_len})")
         dev = self.device
         # The page pool, shared by all layers (a token position occupies the same page id in every
         # layer's cache): slots take pages as they grow and give them back in clear_cache.
