@@ -48,7 +48,8 @@ of the rest, each head its own -- after a prefill chunk, and in decoding when it
 has come to N + ``kv_budget_slack`` (64) tokens, which the device decides for every
 sequence in every step, captured ones included.  ``kv_offset`` then counts the tokens
 in the cache; the caller's position ids are its own.  A slot needs pages for N tokens plus the
-longest chunk or the slack.
+longest chunk or the slack, whichever is more: a chunk that would not fit behind what
+the slack has let grow finds the sequence cut first.
 Prefill writes its rows and the mean keys of the pages it completes with the
 ragged append kernel and attends to the slot's pages with the chunk attention
 kernel (LiteSys calls flashinfer there, batch_cache.py:112-145).
@@ -337,19 +338,27 @@ class PagedBatchKVManager:
         offset = int(self.kv_offset[layer_idx][slot].item())
         total = offset + seq_len
         pad = self.pad                                   # token t lives in cache slot t + pad
-        if total + pad > self.pages_per_slot * self.page:
+        room = self.pages_per_slot * self.page - pad
+        cut_first = self.kv_budget is not None and self.kv_budget < offset <= room < total
+        if cut_first:
+            total = self.kv_budget + seq_len
+        if total > room:
             raise ValueError(f"sequence of {total} tokens exceeds max_seq_len")
         Hkv, D = self.num_key_value_heads, self.head_dim
         n_pages = (total + pad + self.page - 1) // self.page
         self._step_batch_idx = None   # the next decode step builds its table afresh
-        self.pool.reserve(torch.tensor([total + pad], dtype=torch.int32, device=self.device),
-                          torch.tensor([slot], dtype=torch.int32, device=self.device))
+        slots = torch.tensor([slot], dtype=torch.int32, device=self.device)
+        self.pool.reserve(torch.tensor([total + pad], dtype=torch.int32, device=self.device), slots)
         free, bits = self.pool.status()
         if bits & ops.PagePool.EXHAUSTED:
             # nothing was reserved and nothing is recorded: the request can be retried after a clear_cache
             self.pool.acknowledge()
             raise _lib.KineticsError(f"page pool exhausted ({free} pages free): cannot hold {total} tokens in slot {slot}")
-        self.kv_offset[layer_idx][slot] += seq_len
+        if cut_first:
+            held = self.pool.slot_table[slot, :(offset + self.page - 1) // self.page].contiguous()
+            self._evict(layer_idx, held, torch.tensor([0, held.numel()], dtype=torch.int32, device=self.device),
+                        torch.tensor([offset - (held.numel() - 1) * self.page], dtype=torch.int32, device=self.device), slots)
+        self.kv_offset[layer_idx][slot] = total
         idx = self.pool.slot_table[slot, :n_pages].contiguous()
         ptr = torch.tensor([0, n_pages], dtype=torch.int32, device=self.device)
         last = torch.tensor([total + pad - (n_pages - 1) * self.page], dtype=torch.int32, device=self.device)
@@ -362,7 +371,6 @@ class PagedBatchKVManager:
         lse = None if self.kv_budget is None else torch.empty(seq_len, self.num_attention_heads, device=self.device)
         o = ops.paged_chunk_attention(q, self.kv_cache[layer_idx], rows, idx, ptr, last, n_pages, lse=lse, first_page_offset=pad)
         if self.kv_budget is not None:
-            slots = torch.tensor([slot], dtype=torch.int32, device=self.device)
             ops.attention_mass(q, self.kv_cache[layer_idx], lse, self.scores[layer_idx], rows, idx, ptr, last, n_pages, slot_ids=slots)
             if total > self.kv_budget:
                 self._evict(layer_idx, idx, ptr, last, slots)
