@@ -368,7 +368,7 @@ class PagedBatchKVManager:
                                    self.kv_cache[layer_idx], self.kbar[layer_idx][slot:slot + 1], idx, ptr, last)
         # causal with the slot's history, straight from its pages
         q = query_states[0].transpose(0, 1).contiguous()                                       # [s, Hq, D]
-        lse = None if self.kv_budget is None else torch.empty(seq_len, self.num_attention_heads, device=self.device)
+        lse = None if self.kv_budget is None else torch.empty(seq_len, self.num_attention_heads, dtype=torch.float32, device=self.device)
         o = ops.paged_chunk_attention(q, self.kv_cache[layer_idx], rows, idx, ptr, last, n_pages, lse=lse, first_page_offset=pad)
         if self.kv_budget is not None:
             ops.attention_mass(q, self.kv_cache[layer_idx], lse, self.scores[layer_idx], rows, idx, ptr, last, n_pages, slot_ids=slots)

@@ -1,4 +1,5 @@
-"""The KV manager with a budget in slots that have just enough room."""
+"""The KV manager with a budget in slots that have just enough room, and under another default dtype."""
+import math
 from types import SimpleNamespace
 
 import pytest
@@ -95,3 +96,19 @@ def test_a_chunk_that_cannot_fit_changes_nothing():
     grown(m, 1, 80)
     T.prefill(m, 0, 40)                              # 5 + 3 pages: the pool is used up
     unchanged(60)                                    # would be cut to 64 first, but there are no pages for 124 tokens
+
+
+@pytest.mark.gpu
+def test_prefill_under_another_default_dtype():
+    """Model loaders set the default dtype; the log-sum-exp is fp32 whatever it is."""
+    torch.manual_seed(7)
+    m = T.manager(slack=8)
+    q, k, v = T.fresh(1, T.HQ, 100, T.D), T.fresh(1, T.HKV, 100, T.D), T.fresh(1, T.HKV, 100, T.D)
+    old = torch.get_default_dtype()
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        out = m.compute_attention(q, k, v, 0, torch.tensor([0], device=DEV))
+    finally:
+        torch.set_default_dtype(old)
+    want, _, tol = T.attend(q[0], k[0].double(), v[0].double())
+    assert bool(((out[0].double() - want).abs() <= tol).all()) and math.isfinite(float(m.scores[0].sum()))
