@@ -39,6 +39,7 @@ struct ChunkParams {
   float scale_log2;               // sm_scale * log2 e
   float cap_in, cap_log2;         // sm_scale / cap, cap * log2 e (cap_log2 == 0: no cap)
   float cap_tiny[4];              // scale_log2 * kTanhTinyPoly[i] * cap_in^(2i): a small capped score straight from the raw product
+  float cap_tiny_top;             // below this part of the cap: kTanhTiny; 0 where cap_tiny leaves fp32's range
 };
 
 // One sequence of the batch as the kernels see it; positions are token indices.
@@ -117,7 +118,7 @@ __device__ __forceinline__ void cap_scores(const ChunkParams& p, floatx16& s, Mi
 #pragma unroll
   for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(s[e]));
   top *= p.cap_in;
-  if (!__ballot(!(top < kTanhTiny))) {
+  if (!__ballot(!(top < (READY ? p.cap_tiny_top : kTanhTiny)))) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       if constexpr (READY) {

@@ -721,7 +721,12 @@ void fill_chunk_params(ChunkParams& p, const void* q, const void* kv_cache, cons
   p.cap_in = softcap > 0.f ? scale / softcap : 0.f;
   p.cap_log2 = softcap > 0.f ? (float)((double)softcap * 1.4426950408889634) : 0.f;
   double power = (double)scale * 1.4426950408889634;
-  for (int i = 0; i < 4; ++i, power *= (double)p.cap_in * p.cap_in) p.cap_tiny[i] = (float)(power * kTanhTinyPoly[i]);
+  p.cap_tiny_top = kTanhTiny;
+  for (int i = 0; i < 4; ++i, power *= (double)p.cap_in * p.cap_in) {
+    p.cap_tiny[i] = (float)(power * kTanhTinyPoly[i]);
+    // An infinite coefficient would make NaN of a score of 0, one that is lost changes the others: the next form then.
+    if (!std::isnormal(p.cap_tiny[i])) p.cap_tiny_top = 0.f;
+  }
 }
 
 // Row tiles of the launch, and the spans into which their keys are cut.
