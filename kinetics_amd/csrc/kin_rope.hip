@@ -106,7 +106,10 @@ __global__ __launch_bounds__(256) void qkv_norm_rope_kernel(RopeParams p) {
     }
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = fmaf(x[i], c[i], __shfl_xor(x[i], LPR / 2) * s[i]);
+    for (int i = 0; i < 8; ++i) {
+      const float other = __shfl_xor(x[i], LPR / 2);
+      y[i] = fmaf(x[i], c[i], s[i] == 0.f ? 0.f : other * s[i]);  // not turned: an infinite partner is no part of it
+    }
     u32x4* dst = is_q ? p.q + ((int64_t)t * p.hq + j) * LPR : p.k + ((int64_t)t * p.hkv + (j - p.hq)) * LPR;
     dst[l] = pack8<F16>(y);
   }

@@ -1,4 +1,6 @@
 """The chunk operators at the ends of their ranges."""
+import math
+
 import pytest
 import torch
 
@@ -23,3 +25,26 @@ def test_mass_of_scores_of_zero_under_any_cap(softcap, news):
     got = start.clone()
     ops.attention_mass(pb.q, pb.kv, lse, got, pb.q_indptr, pb.ids, pb.ptr, pb.last, pb.max_pages, softcap=softcap)
     assert bool(((got.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("d", [128, 64])
+def test_a_pair_that_is_not_turned_keeps_its_elements(d, dtype):
+    """Whatever its partner is: an infinity or NaN in the other half is no part of it."""
+    from kinetics_amd import ops
+
+    g = torch.Generator().manual_seed(2)
+    qkv = torch.randn(5, 6 * d, generator=g).to(R.DT[dtype]).to(DEV)
+    x = qkv.view(5, 6, d)
+    x[0, 0, d // 2 - 1], x[1, 4, d - 1], x[2, 3, d - 2] = math.inf, math.nan, -math.inf
+    freq, axis = ops.rope_table(d, sections=[3], device=DEV)
+    pos = torch.arange(5, dtype=torch.int32, device=DEV) * 7
+    q, k, v = ops.qkv_norm_rope_split(qkv, None, None, 1e-6, pos, freq, axis, 4, 1)
+    got = torch.cat([q, k, v], 1).double()
+    same = [i for i in range(d) if i % (d // 2) >= 3]
+    assert torch.equal(got[:, :, same].nan_to_num(nan=7e7), x[:, :, same].double().nan_to_num(nan=7e7))
+    want = R.rope(qkv, None, None, 1e-6, pos, [1e6 ** (-2.0 * i / d) for i in range(d // 2)], axis.tolist(), 4, 1, d)
+    turned = [i for i in range(d) if i % (d // 2) < 3]
+    mag = x[:, :5].double().abs().nan_to_num(0, 0, 0).amax(-1, keepdim=True) * 1.5
+    err = (got[:, :5] - torch.cat(want[:2], 1)).abs()[..., turned]
+    assert bool((err <= (torch.finfo(R.DT[dtype]).eps / 2 + 2.0 ** -18) * mag).all())
