@@ -802,12 +802,14 @@ static int chunk_attention_impl(const char* fn, bool f16, const void* q, const v
   if (batch == 0 || nnz == 0) return KIN_OK;
   ChunkAttnParams ap;
   const int64_t slots = chunk_slots(nnz, batch, num_q_heads / num_kv_heads);
-  if (slots * num_kv_heads > 0x7fffffffLL) return fail(KIN_ERR_UNSUPPORTED, "%s: too many row tiles", fn);
+  if (slots * num_kv_heads > max_workgroups(256)) return fail(KIN_ERR_UNSUPPORTED, "%s: too many row tiles", fn);
   const ChunkSpans spans = chunk_spans(nnz, batch, num_q_heads, num_kv_heads, max_pages_per_seq, page_size, head_dim, num_splits);
   ap.num_splits = spans.splits;
   ap.span_narrow = spans.narrow;
   ap.span_wide = spans.wide;
   if (ap.num_splits > 1) {
+    if (nnz * num_q_heads > max_workgroups(256) * (1024 / head_dim))  // the join
+      return fail(KIN_ERR_UNSUPPORTED, "%s: nnz*num_q_heads is too large for %d splits", fn, ap.num_splits);
     const size_t need = chunk_workspace(nnz, num_q_heads, head_dim, ap.num_splits);
     if (!workspace || workspace_bytes < need)
       return fail(KIN_ERR_WORKSPACE, "%s: %d splits need %zu workspace bytes, got %zu", fn, ap.num_splits, need,

@@ -55,6 +55,8 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));  // one 16-byte 
 int fail(int status, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int check_hip(hipError_t e, const char* what);
 
+// Most workgroups of `threads` threads that one dimension of a launch can have: it holds fewer than 2^32 threads.
+constexpr int64_t max_workgroups(int threads) { return 0xffffffffLL / threads; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Shape rules every entry point shares.  Returns KIN_OK or records an error.

@@ -336,7 +336,8 @@ static int evict_tokens_impl(const char* fn, void* kv_cache, const float* scores
   int part_bytes = 128;
   while (part_bytes > 32 && lists * (head_dim * 2 / part_bytes) < kNumCus) part_bytes /= 2;
   const int parts = head_dim * 2 / part_bytes;
-  if (lists * parts > 0x7fffffffLL)
+  // both kernels before either is launched
+  if (lists * parts > max_workgroups(kMoveThreads) || (int64_t)batch * num_kv_heads > max_workgroups(kEvictThreads))
     return fail(KIN_ERR_UNSUPPORTED, "%s: batch*num_kv_heads is too large", fn);
   if (batch == 0) return KIN_OK;
   EvictParams p;

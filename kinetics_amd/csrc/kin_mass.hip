@@ -241,11 +241,14 @@ static int attention_mass_impl(const char* fn, bool f16, const void* q, const vo
   mp.slot_ids = slot_ids;
   mp.num_blocks = score_blocks;
   mp.stride = score_stride;
-  mp.key_tiles = (int)(((int64_t)max_pages_per_seq * page_size + kMassKeys - 1) / kMassKeys);
-  const int64_t grid = (int64_t)batch * num_kv_heads * mp.key_tiles;
-  if (grid > 0x7fffffffLL) return fail(KIN_ERR_UNSUPPORTED, "%s: batch*num_kv_heads*max_pages_per_seq is too large", fn);
   const bool extra = slopes != nullptr || softcap > 0.f;
   const bool many_rows = nnz * mp.c.group > 64 * (int64_t)batch;  // on average more than a stage of the small form
+  // A workgroup for every tile of the longest page list, or as many as a launch can have: they walk on.
+  const int64_t lists = (int64_t)batch * num_kv_heads, most = max_workgroups(many_rows ? 512 : 256) / lists;
+  if (most < 1) return fail(KIN_ERR_UNSUPPORTED, "%s: batch*num_kv_heads=%lld is too large", fn, (long long)lists);
+  const int64_t tiles = ((int64_t)max_pages_per_seq * page_size + kMassKeys - 1) / kMassKeys;
+  mp.key_tiles = (int)(tiles < most ? tiles : most);
+  const int64_t grid = lists * mp.key_tiles;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (head_dim == kHeadDimSmall) {
     if (f16) launch_mass<kHeadDimSmall, true>(mp, (unsigned)grid, extra, many_rows, s);

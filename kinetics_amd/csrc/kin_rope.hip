@@ -115,10 +115,11 @@ __global__ __launch_bounds__(256) void qkv_norm_rope_kernel(RopeParams p) {
   }
 }
 
+// Few heads: four tokens a workgroup, so that its threads have rows to take.
+static int tokens_per_workgroup(int hq, int hkv, int lanes_per_row) { return ((int64_t)hq + 2 * (int64_t)hkv) * lanes_per_row <= 128 ? 4 : 1; }
 template <bool F16, int LPR, bool NORM>
 static void launch_rope(const RopeParams& p, hipStream_t s) {
-  // Few heads: four tokens a workgroup, so that its threads have rows to take.
-  if ((p.hq + 2 * p.hkv) * LPR <= 128) qkv_norm_rope_kernel<F16, LPR, 4, NORM><<<(unsigned)((p.tokens + 3) / 4), 256, 0, s>>>(p);
+  if (tokens_per_workgroup(p.hq, p.hkv, LPR) == 4) qkv_norm_rope_kernel<F16, LPR, 4, NORM><<<(unsigned)((p.tokens + 3) / 4), 256, 0, s>>>(p);
   else qkv_norm_rope_kernel<F16, LPR, 1, NORM><<<(unsigned)p.tokens, 256, 0, s>>>(p);
 }
 
@@ -135,6 +136,8 @@ static int qkv_norm_rope_impl(const char* fn, bool f16, const void* qkv, int64_t
     return fail(KIN_ERR_UNSUPPORTED, "%s: head_dim=%d, only %d and %d are built", fn, head_dim, kHeadDimSmall, kHeadDim);
   const int64_t width = ((int64_t)num_q_heads + 2 * (int64_t)num_kv_heads) * head_dim;
   if (width > 0x7fffffffLL) return fail(KIN_ERR_UNSUPPORTED, "%s: too many heads", fn);
+  if (tokens > max_workgroups(256) * tokens_per_workgroup(num_q_heads, num_kv_heads, head_dim / 8))
+    return fail(KIN_ERR_UNSUPPORTED, "%s: tokens=%d are too many for a call", fn, tokens);
   if (qkv_row_stride < width || qkv_row_stride % 8 != 0)
     return fail(KIN_ERR_BAD_SHAPE, "%s: qkv_row_stride=%lld must be a multiple of 8 and at least the row width %lld", fn,
                 (long long)qkv_row_stride, (long long)width);

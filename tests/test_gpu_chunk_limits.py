@@ -48,3 +48,20 @@ def test_a_pair_that_is_not_turned_keeps_its_elements(d, dtype):
     mag = x[:, :5].double().abs().nan_to_num(0, 0, 0).amax(-1, keepdim=True) * 1.5
     err = (got[:, :5] - torch.cat(want[:2], 1)).abs()[..., turned]
     assert bool((err <= (torch.finfo(R.DT[dtype]).eps / 2 + 2.0 ** -18) * mag).all())
+
+
+def test_mass_of_many_long_page_lists():
+    """512 sequences of 8 heads planned for 2^22 tokens each: more (sequence, head, tile) triples than a grid holds workgroups."""
+    from kinetics_amd import ops
+
+    lens = [0] * 512
+    lens[3], lens[511] = 700, 40
+    news = [0] * 512
+    news[3], news[511] = 2, 1
+    pb = R.problem(3, lens, news, 8, 8, 64, 16, "bf16")
+    lse = torch.empty(pb.q.shape[:2], device=DEV)
+    ops.paged_chunk_attention(pb.q, pb.kv, pb.q_indptr, pb.ids, pb.ptr, pb.last, pb.max_pages, lse=lse)
+    start = torch.rand(512, 8, 704, device=DEV)
+    want, tol = R.mass(pb, lse, start)
+    ops.attention_mass(pb.q, pb.kv, lse, start, pb.q_indptr, pb.ids, pb.ptr, pb.last, 2 ** 18)
+    assert bool(((start.double() - want).abs() <= tol).all())
