@@ -756,9 +756,11 @@ size_t kin_chunk_workspace_bytes(int64_t nnz, int batch, int num_q_heads, int nu
  *   out[r, g, :] = sum_j softmax_j(s)[j] * v_j,   lse[r, g] = log sum_j exp(s_j)
  * over the seen tokens; a row that sees none gives zeros and -inf.  lse (fp32
  * [nnz, num_q_heads], natural logarithm) may be NULL.  Scores, softmax and sums
- * are fp32; weights are rounded to the cache's element type before the product
- * with V, as the result is.  num_splits 0: chosen from the sizes.  Calls that
- * may overlap in time need workspaces of their own.
+ * are fp32.  Before the product with V, weights are rounded to the cache's element
+ * type, as the result is, where a sequence's new rows (times query heads of a KV
+ * head) fill more than 32 of a tile of 128; up to 32 rows, as in decoding, they are
+ * kept to 2^-18.  num_splits 0: chosen from the sizes.  Calls that may overlap in time
+ * need workspaces of their own.
  */
 int kin_paged_chunk_attention(const kin_bf16_t* q, const kin_bf16_t* kv_cache, const int32_t* q_indptr,
                               const int32_t* page_indices, const int32_t* page_indptr,

@@ -14,9 +14,12 @@
 // O^T += V^T P^T wants P with 8 consecutive registers per lane as the matrix unit's operand; the
 // registers hold the keys 4h + 0..3 and 8 + 4h + 0..3 (h = lane / 32) of every 16, and as the order in
 // which keys are summed is free, V^T is read in that same order: ds_read_b64_tr_b16 hands a lane
-// four keys of one column.  P never leaves the registers.  P is rounded to the cache's element type
-// for the matrix unit (half a unit in the last place, as the result itself); the running sum and
-// maximum, and O, are fp32.
+// four keys of one column.  P never leaves the registers.  The running sum and maximum, and O, are fp32.
+//
+// The matrix unit takes P in the cache's element type.  With more than 32 rows a weight is rounded to it once (half a unit in the
+// last place, as the result itself): a second element for what the rounding leaves makes half as many products again, 550 -> 750 us
+// for 8192 tokens from nothing and 155 -> 219 for 2048 behind 30720, which the matrix unit bounds.  With up to 32 rows, where it waits for HBM,
+// it gets both: 2^-18 of a bfloat16 weight is left, as in the decode kernels' fp32 (60 single tokens beside four prompts 129.2 -> 130.5 us).
 //
 // What bounds it, measured in bf16 on MI355X: prompts the matrix unit (51 % busy), the LDS reads and the softmax together --
 // 8192 tokens from nothing, 32 heads on 8 of 128: 546 us, 1.0 PFLOP/s; 2048 behind 30720, 4 heads on 1: 155 us, 0.86 PFLOP/s.
@@ -45,6 +48,7 @@ struct ChunkAttnParams {
 };
 
 typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
 
 // First row tile of the sequence b whose rows start at e0: tiles are numbered so that every sequence has room for its rows
 // whatever the others bring, without a scan: floor(e0 * group / 128) + b.
@@ -111,16 +115,6 @@ __device__ __forceinline__ void load_rows(const ChunkParams& p, const ChunkSeq& 
   for (int k = 0; k < HD / 16; ++k) w.q[k] = valid ? src[2 * k + half] : uint4{0, 0, 0, 0};
 }
 
-// Any element of the 8 that is infinite or NaN?
-template <bool F16>
-__device__ __forceinline__ bool any_special(const uint4& v) {
-  const uint32_t e = F16 ? 0x7c00u : 0x7f80u;
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  bool any = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) any |= (w[i] & e) == e || ((w[i] >> 16) & e) == e;
-  return any;
-}
 // The 8 elements with zeros in place of the infinite and NaN ones.
 template <bool F16>
 __device__ __forceinline__ uint4 finite_only(const uint4& v) {
@@ -233,18 +227,25 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
     for (int dt = 0; dt < HD / 32; ++dt) early[dt] = read_v(0, 0, dt);
     __builtin_amdgcn_sched_barrier(0);
   }
-  uint4 pb[NSUB][2];
+  // Up to 32 rows: a weight as two elements, the second what the first one's rounding left.
+  constexpr bool kTwoParts = NSUB == 1;
+  uint4 pb[NSUB][2], pl[2];
 #pragma unroll
   for (int t = 0; t < NSUB; ++t) {
-    uint32_t d[8];
+    uint32_t d[8], r[8];
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
       const float p0 = fast_exp2(fmaf(s[t][e], c, -shift)), p1 = fast_exp2(fmaf(s[t][e + 1], c, -shift));
       w.l += p0 + p1;
       d[e / 2] = pack2<F16>(p0, p1);
+      if constexpr (kTwoParts) r[e / 2] = pack2<F16>(p0 - elem_lo<F16>(d[e / 2]), p1 - elem_hi<F16>(d[e / 2]));
     }
     pb[t][0] = uint4{d[0], d[1], d[2], d[3]};
     pb[t][1] = uint4{d[4], d[5], d[6], d[7]};
+    if constexpr (kTwoParts) {
+      pl[0] = uint4{r[0], r[1], r[2], r[3]};
+      pl[1] = uint4{r[4], r[5], r[6], r[7]};
+    }
   }
   before_v();
   if constexpr (!EXTRA) __builtin_amdgcn_s_setprio(1);
@@ -258,19 +259,26 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
         if constexpr (kEarlyValues) a = t == 0 && kk == 0 ? early[dt] : read_v(t, kk, dt);
         else a = read_v(t, kk, dt);
         w.o[dt] = mfma_32x32x16<F16>(a, pb[t][kk], w.o[dt]);
+        if constexpr (kTwoParts) w.o[dt] = mfma_32x32x16<F16>(a, pl[kk], w.o[dt]);
       }
   if constexpr (!EXTRA) __builtin_amdgcn_s_setprio(0);
 }
 
-// A value that is not seen has weight 0, and 0 times an infinity would be NaN.  In the blocks where some row does not see
-// some key, infinite and NaN values are therefore taken out of the staged rows: which elements of this
+// A value that is not seen has weight 0, and 0 times an infinity would be NaN; so would be the sum of a weight's two parts
+// times an infinity.  In the blocks where some row does not see some key, and in all blocks where weights have two
+// parts, infinite and NaN values are therefore taken out of the staged rows: which elements of this
 // lane's output they reach is kept as bits, and the result gets them at the end.
-template <int HD, bool F16>
-__device__ __forceinline__ bool rows_special(const unsigned char* v, int rows) {
-  bool any = false;
-#pragma unroll 1
-  for (int x = threadIdx.x & 63; x < rows * (HD / 8); x += 64) any |= any_special<F16>(*reinterpret_cast<const uint4*>(v + x * 16));
-  return __ballot(any) != 0;
+template <int HD, bool F16, int ROWS>
+__device__ __forceinline__ bool rows_special(const unsigned char* v) {
+  ushortx2 top = {0, 0};  // the largest magnitude bits of the even and of the odd elements
+#pragma unroll
+  for (int x = 0; x < ROWS * (HD / 8); x += 64) {
+    const uint4 y = *reinterpret_cast<const uint4*>(v + (x + (threadIdx.x & 63)) * 16);
+    const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(ushortx2, w[i] & 0x7fff7fffu));
+  }
+  return __ballot(max(top.x, top.y) >= (F16 ? 0x7c00 : 0x7f80)) != 0;
 }
 template <int HD, bool F16>
 __device__ __forceinline__ void note_specials(WaveRows<HD>& w, const unsigned char* v, int keys, int slot0, uint32_t units, int first) {
@@ -440,7 +448,7 @@ __global__ __launch_bounds__(256, chunk_wgs_per_cu(HD)) void chunk_attn_kernel(C
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(wait_vm_imm(HD / 16));  // the values are in; the next keys may be on their way
         __builtin_amdgcn_sched_barrier(0);
-        if (masked && rows_special<HD, F16>(vbuf, 32)) {
+        if (rows_special<HD, F16, 32>(vbuf)) {
           note_specials<HD, F16>(w, vbuf, 32, slot0, units, off);
           clear_specials<HD, F16>(vbuf, 32);
         }
@@ -551,7 +559,7 @@ __global__ __launch_bounds__(256, chunk_wgs_per_cu(HD)) void chunk_attn_kernel(C
     if (it + 1 < it1) stage_tile(it + 1, lds + (1 - stage) * kStageB, units_next);
     const int slot0 = tile_at(it) * kChunkKeys;
     if (!seen_whole(slot0, units, pos0, pos1)) {  // the whole workgroup looks for infinite and NaN values
-      const bool any = rows_special<HD, F16>(vst + wave * kUnitB, 16);
+      const bool any = rows_special<HD, F16, 16>(vst + wave * kUnitB);
       if (lane == 0) sm_m[0][wave] = any ? 1.f : 0.f;
       __syncthreads();
       if (sm_m[0][0] + sm_m[0][1] + sm_m[0][2] + sm_m[0][3] > 0.f) {
