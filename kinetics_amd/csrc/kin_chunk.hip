@@ -33,7 +33,16 @@ constexpr int kChunkRows = 128;     // rows of a workgroup's tile
 constexpr int kChunkKeys = 64;      // keys of a staged tile
 // Workgroups on a CU: the registers of a wave's outputs allow 3 with heads of 64 and 2 with heads of 128.
 constexpr int chunk_wgs_per_cu(int head_dim) { return head_dim == kHeadDimSmall ? 3 : 2; }
-constexpr float kRescaleLog2 = 8.f; // the running maximum is only moved when a score passes it by 2^8
+// A weight is 2^(score - reference + up): the reference, the running maximum, is only moved when a score passes it by
+// rescale_at.  bfloat16 has fp32's range.  float16 ends at 2^16 and in steps of 2^-24: with weights of up to 2^15, one of 2^-27 of the
+// reference has all its bits and none above 2^-38 is lost (at 2^0, thousands of 2^-26 were in the sum but not in the result).
+// Scores above 2^20 are too coarse for that: fp32 may take one above its reference by more than float16 has left.
+constexpr float rescale_at(bool f16) { return f16 ? 2.f : 8.f; }
+template <bool F16>
+__device__ __forceinline__ float weight_up(float reference) {
+  if constexpr (F16) return fabsf(reference) < 0x1p20f ? 13.f : 0.f;
+  return 0.f;
+}
 
 struct ChunkAttnParams {
   ChunkParams c;
@@ -92,6 +101,7 @@ struct WaveRows {
   uint4 q[HD / 16];
   floatx16 o[HD / 32];
   float m, l;       // running maximum (units of the raw product, or log2 with EXTRA) and this lane's part of the sum
+  float up;         // its weights are larger by 2^up
   RowSpan span;
   float slope2;
   uint64_t pos_inf, neg_inf;  // bit e: output register e gets an infinity of that sign (both: NaN)
@@ -102,7 +112,7 @@ __device__ __forceinline__ void load_rows(const ChunkParams& p, const ChunkSeq& 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int i = r / p.group, g = r - i * p.group;
   w.m = kNegInf;
-  w.l = 0.f;
+  w.l = w.up = 0.f;
   w.pos_inf = w.neg_inf = 0;
 #pragma unroll
   for (int t = 0; t < HD / 32; ++t)
@@ -189,20 +199,20 @@ __device__ __forceinline__ void attend_block(const ChunkParams& p, WaveRows<HD>&
 #pragma unroll
     for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[t][e]);
   mt = max_halves(EXTRA ? mt + bias : mt);
-  // The reference maximum follows the scores only when they pass it by 2^8 (weights stay below 2^8, which both
-  // element types and the fp32 sums hold without loss), so most blocks need no rescaling of O.
-  const bool move = mt > w.m && !((mt - w.m) * c <= kRescaleLog2);
+  // The reference follows the scores only when they pass it by some way, so most blocks need no rescaling of O.
+  const bool move = mt > w.m && !((mt - w.m) * c <= rescale_at(F16));
   if (__ballot(move)) {
-    const float m_new = move ? mt : w.m;
-    const float alpha = m_new == kNegInf ? 1.f : fast_exp2((w.m - m_new) * c);
+    const float m_new = move ? mt : w.m, up = move ? weight_up<F16>(mt * c) : w.up;
+    const float alpha = m_new == kNegInf ? 1.f : fast_exp2((w.m - m_new) * c + (up - w.up));
     w.m = m_new;
+    w.up = up;
     w.l *= alpha;
 #pragma unroll
     for (int t = 0; t < HD / 32; ++t)
 #pragma unroll
       for (int e = 0; e < 16; ++e) w.o[t][e] *= alpha;
   }
-  const float shift = (w.m == kNegInf ? 0.f : w.m * c) - (EXTRA ? bias : 0.f);
+  const float shift = (w.m == kNegInf ? 0.f : w.m * c) - w.up - (EXTRA ? bias : 0.f);
   // V^T: lane (16-lane group g = lane / 16 % 2, place q = lane % 16) asks for 4 columns of key row q / 4 and is handed
   // the 4 keys of column 16 g + q; two such reads make one operand (keys 4h.. and 8 + 4h..).
   const int q4 = (lane & 15) >> 2, cq = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), lo8 = (lane & 1) * 8;
@@ -469,7 +479,7 @@ __global__ __launch_bounds__(256, chunk_wgs_per_cu(HD)) void chunk_attn_kernel(C
     const float c = EXTRA ? 1.f : p.scale_log2;
     __syncthreads();
     if (lane < 32) {
-      sm_m[wave][lane] = w.m == kNegInf ? kNegInf : w.m * c;
+      sm_m[wave][lane] = w.m == kNegInf ? kNegInf : w.m * c - w.up;
       sm_l[wave][lane] = w.l;
     }
     float* ow = reinterpret_cast<float*>(lds);  // [4 waves][rows][HD]
@@ -581,7 +591,7 @@ __global__ __launch_bounds__(256, chunk_wgs_per_cu(HD)) void chunk_attn_kernel(C
     const float l = w.l + other_half(w.l);
     const bool none = w.m == kNegInf && l == 0.f;
     const float inv = none ? 0.f : 1.f / l;
-    const float lse2 = none ? kNegInf : w.m * c + __log2f(l);
+    const float lse2 = none ? kNegInf : w.m * c + (__log2f(l) - w.up);
     const int i = (r0 + row) / p.group, g = (r0 + row) - i * p.group;
     const int64_t hq = (int64_t)(sq.e0 + i) * p.hq + h * p.group + g;
     const int64_t at = (int64_t)split * p.nnz * p.hq + hq;

@@ -91,6 +91,48 @@ def test_few_rows(ops, dtype, lens, news, hq, hkv, d, page, offset):
     check(pb, attend(ops, pb, **mods), **mods)
 
 
+@pytest.mark.parametrize("news", [1, 5, 64, 200])
+@pytest.mark.parametrize("extra", [False, True])
+def test_many_small_weights_in_float16(ops, news, extra):
+    """One heavy token with a value of 0 and thousands of weight 2^-26: their values are the whole result."""
+    n = 4000
+    pb = R.problem(3, [n], [news], 4, 1, 128, 16, "f16")
+    page, slot = R.slot_of(pb, 0, torch.arange(n, device=DEV))
+    k, v = torch.zeros(n, 128, dtype=pb.dt, device=DEV), torch.full((n, 128), 1000.0, dtype=pb.dt, device=DEV)
+    k[0, 0], v[0] = 25.75, 0.0
+    v[1:, 64:] *= 1 + torch.rand(n - 1, 64, device=DEV).to(pb.dt)
+    pb.kv[page, 0, slot, 0], pb.kv[page, 1, slot, 0] = k, v
+    pb.q.zero_()
+    pb.q[:, :, 0] = torch.tensor([8.0, 7.5, 4.0, 8.25], device=DEV, dtype=pb.dt)
+    mods = dict(softcap=200.0) if extra else {}
+    check(pb, attend(ops, pb, **mods), narrow=news * 4 <= 32, **mods)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("news", [1, 40])
+@pytest.mark.parametrize("power", [6, 9, 11, 12, 13, 14, 15])
+def test_scores_of_many_millions(ops, power, news, dtype):
+    """Far apart, so that every row gets the value of its largest score, whatever fp32 makes of its last digits."""
+    n = 700
+    pb = R.problem(6, [n], [news], 4, 1, 128, 16, dtype)
+    g = torch.Generator().manual_seed(6)
+    step = 64 + 64 * torch.randperm(n, generator=g).to(DEV)                  # up to 44864, some not exact in 16 bits
+    page, slot = R.slot_of(pb, 0, torch.arange(n, device=DEV))
+    k = torch.zeros(n, 128, dtype=pb.dt, device=DEV)
+    k[:, 0] = step.to(pb.dt)
+    pb.kv[page, 0, slot, 0] = k
+    pb.q.zero_()
+    pb.q[:, :, 0] = torch.tensor([1.0, -1.0, 0.5, 0.75], device=DEV, dtype=pb.dt) * 2.0 ** power
+    got = attend(ops, pb)
+    v = pb.kv[page, 1, slot, 0]
+    for r in range(news):
+        for head in range(4):
+            s = k[:n - news + r + 1, 0].double() * float(pb.q[r, head, 0])
+            top = (s == s.max()).nonzero()[:, 0]
+            want = v[top].double().mean(0)
+            assert bool(((got[r, head].double() - want).abs() <= torch.finfo(pb.dt).eps * (want.abs() + v[top].double().abs().amax(0))).all())
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("news", [1, 7, 60])
 def test_infinite_values_that_every_row_sees(ops, news, dtype):
