@@ -6,9 +6,9 @@
 // 35 us, 5.8 TB/s; 4096 tokens of 4 + 2 heads: 6 us).
 //
 // Positions run to millions, where an fp32 angle has no digits left behind the full turns.  Frequencies are
-// therefore turns per position as 64-bit fractions: position times fraction, modulo 2^64, IS the angle
-// modulo a full turn, exactly, in integer arithmetic; its upper 32 bits go to fp32 as a signed part of a turn
-// (2^-26 of a turn off at most) and sincospi does the rest.  The D/2 angles of a token are taken once and
+// therefore turns per position as 64-bit fractions: position times fraction, modulo 2^64, IS the angle of that
+// fraction modulo a full turn, exactly, in integer arithmetic; its upper 32 bits go to fp32 as a signed part of a turn
+// (2^-26 of a turn off at most, and 2^-32 for the lower bits) and sincospi does the rest.  The D/2 angles of a token are taken once and
 // shared by its q and k heads through LDS.
 #include "kin_common.h"
 
@@ -74,11 +74,13 @@ __global__ __launch_bounds__(256) void qkv_norm_rope_kernel(RopeParams p) {
   const int l = in % LPR, row0 = in / LPR;
   const bool upper = l >= LPR / 2;
   float c[8], s[8];
+  uint32_t turned[8];  // the partner's bits, or none where a pair is not turned: 0 times an infinity would be NaN
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float2 z = cs[sub][8 * (l & (LPR / 2 - 1)) + i];
     c[i] = z.x;
     s[i] = upper ? z.y : -z.y;  // lower half: lo c - hi s; upper half: hi c + lo s
+    turned[i] = z.y == 0.f ? 0u : ~0u;
   }
   float wq[8], wk[8];
   if constexpr (NORM) {
@@ -106,10 +108,8 @@ __global__ __launch_bounds__(256) void qkv_norm_rope_kernel(RopeParams p) {
     }
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = __shfl_xor(x[i], LPR / 2);
-      y[i] = fmaf(x[i], c[i], s[i] == 0.f ? 0.f : other * s[i]);  // not turned: an infinite partner is no part of it
-    }
+    for (int i = 0; i < 8; ++i)
+      y[i] = fmaf(x[i], c[i], __uint_as_float(__float_as_uint(__shfl_xor(x[i], LPR / 2)) & turned[i]) * s[i]);
     u32x4* dst = is_q ? p.q + ((int64_t)t * p.hq + j) * LPR : p.k + ((int64_t)t * p.hkv + (j - p.hq)) * LPR;
     dst[l] = pack8<F16>(y);
   }
