@@ -756,11 +756,13 @@ size_t kin_chunk_workspace_bytes(int64_t nnz, int batch, int num_q_heads, int nu
  *   out[r, g, :] = sum_j softmax_j(s)[j] * v_j,   lse[r, g] = log sum_j exp(s_j)
  * over the seen tokens; a row that sees none gives zeros and -inf.  lse (fp32
  * [nnz, num_q_heads], natural logarithm) may be NULL.  Scores, softmax and sums
- * are fp32.  Before the product with V, weights are rounded to the cache's element
- * type, as the result is, where a sequence's new rows (times query heads of a KV
- * head) fill more than 32 of a tile of 128; up to 32 rows, as in decoding, they are
- * kept to 2^-18.  num_splits 0: chosen from the sizes.  Calls that may overlap in time
- * need workspaces of their own.
+ * are fp32.  The rows of a KV head -- a sequence's new tokens times its query
+ * heads -- go in tiles of 128.  In a tile of more than 32, weights are rounded to the
+ * cache's element type before the product with V, as the result is; in one of up to 32
+ * (decoding; also what is left of a prompt) they are kept to 2^-18.  In float16 a
+ * weight below 2^-27 of the row's largest loses bits and one below 2^-38 is lost.
+ * num_splits 0: chosen from the sizes.  Calls that may overlap in time need workspaces
+ * of their own.
  */
 int kin_paged_chunk_attention(const kin_bf16_t* q, const kin_bf16_t* kv_cache, const int32_t* q_indptr,
                               const int32_t* page_indices, const int32_t* page_indptr,
@@ -904,8 +906,8 @@ int kin_qkv_norm_split_f16(const void* qkv, int64_t qkv_row_stride, const void* 
  * time, height and width); axis: int32 [D/2], which axis turns pair i (an entry
  * outside [0, num_axes) leaves the pair as it is); freq: int64 [D/2], turns per
  * position as a fraction of 2^64, i.e. round(frequency[i] / (2 pi) * 2^64)
- * modulo 2^64: position times fraction is the angle modulo a turn, exactly, for every int32
- * position.  q_weight and k_weight both NULL: no norm.
+ * modulo 2^64: the product of position and fraction is exact modulo a turn for every int32
+ * position, then rounded to fp32 (2^-25.9 of a turn at most).  q_weight and k_weight both NULL: no norm.
  */
 int kin_qkv_norm_rope_split(const void* qkv, int64_t qkv_row_stride, const void* q_weight,
                             const void* k_weight, float eps, const int32_t* positions, int num_axes,

@@ -87,8 +87,8 @@ __device__ __forceinline__ bool row_sees(const RowSpan& r, int first, int slot) 
   return ((slot <= r.hi) & (slot >= r.lo)) | ((slot < r.prefix) & (slot >= first));
 }
 
-// tanh to about 3 units in the last place: x P(x^2) with the P of least largest relative error, of degree 3 below 1/4 (3e-9 by
-// its coefficients) and 5 below 3/4 (3e-8; 1.6e-7 with the fp32 roundings); beyond, 1 - 2 / (exp(2x) + 1), which no longer cancels.
+// tanh to about 3 units in the last place: x P(x^2) with the P of least largest relative error, of degree 3 below 1/4 (5.2e-9 by
+// its coefficients, 9.3e-8 with the fp32 roundings) and 5 below 3/4 (6.5e-8; 1.6e-7); beyond, 1 - 2 / (exp(2x) + 1), which no longer cancels.
 constexpr float kTanhTiny = 0.25f, kTanhSmall = 0.75f;
 constexpr double kTanhTinyPoly[4] = {1.0, -0.3333320617675781, 0.13323132693767548, -0.051327724009752274};
 __device__ __forceinline__ float tanh_over_x_small(float t) {

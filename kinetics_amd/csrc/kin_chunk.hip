@@ -19,11 +19,11 @@
 // The matrix unit takes P in the cache's element type.  With more than 32 rows a weight is rounded to it once (half a unit in the
 // last place, as the result itself): a second element for what the rounding leaves makes half as many products again, 550 -> 750 us
 // for 8192 tokens from nothing and 155 -> 219 for 2048 behind 30720, which the matrix unit bounds.  With up to 32 rows, where it waits for HBM,
-// it gets both: 2^-18 of a bfloat16 weight is left, as in the decode kernels' fp32 (60 single tokens beside four prompts 129.2 -> 130.5 us).
+// it gets both, and 2^-18 of a bfloat16 weight is left; the decode kernels keep fp32 (60 single tokens beside four prompts 129.2 -> 130.5 us).
 //
-// What bounds it, measured in bf16 on MI355X: prompts the matrix unit (51 % busy), the LDS reads and the softmax together --
-// 8192 tokens from nothing, 32 heads on 8 of 128: 546 us, 1.0 PFLOP/s; 2048 behind 30720, 4 heads on 1: 155 us, 0.86 PFLOP/s.
-// Decode rows HBM: 60 single tokens of 301..8201 beside four prompts, 8 KV heads of 64: 129 us.  Few rows the chain of
+// What bounds it, measured on MI355X: prompts the matrix unit (52 % busy) and the vector unit (50 %), which two waves a SIMD hardly overlap --
+// 8192 tokens from nothing, 32 heads on 8 of 128, bf16: 550 us, 1.0 PFLOP/s; 2048 behind 30720, 4 heads on 1: 154 us, 0.86 PFLOP/s.
+// Decode rows HBM: 60 single tokens of 301..8201 beside four prompts, 8 KV heads of 64, f16: 132 us.  Few rows the chain of
 // dependent loads: 8 single tokens of 513..4097: 8 us and 4 for the join.
 #include "kin_chunk.h"
 

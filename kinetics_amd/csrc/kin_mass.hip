@@ -3,12 +3,13 @@
 //                      exp(s_pgj - lse_pg),
 // with the scores s of kin_chunk.h and the log-sum-exp that the attention over the same chunk wrote.
 //
-// A workgroup owns 128 tokens of one (sequence, KV head), each of its 4 waves 32 of them: their keys are read
+// A workgroup owns 128 tokens of one (sequence, KV head), each of four waves 32 of them: their keys are read
 // once and stay in registers as the matrix unit's operand, and the rows pass by, 64 at a time, through two
-// stages in LDS that all four waves read.  S = Q K^T on v_mfma_f32_32x32x16 leaves lane l the scores of ONE token (column l % 32) against
+// stages in LDS that all four waves read.  With many rows (RW = 2) there are eight waves, two for the same 32 tokens, and 128 rows to a
+// stage: each of the two takes every other 32 rows, and their sums are added at the end.  S = Q K^T on v_mfma_f32_32x32x16 leaves lane l the scores of ONE token (column l % 32) against
 // 16 rows, so the sum over rows is a sum over registers: no atomics, one owner per token, and the order of
 // the additions never changes.  With many rows the vector unit bounds it, one exponential and seven slots per (row, token) with a
-// cap: 2048 rows of 8192 tokens, 32 heads on 8: 222 us.  With single tokens it is the reading of the keys: 256 sequences of
+// cap: 2048 rows of 8192 tokens, 32 heads on 8: 230 us, the vector unit 79 % busy.  With single tokens it is the reading of the keys: 256 sequences of
 // 1025..8193, 83 us, 3.7 TB/s.  (Rows straight from L2 instead of through LDS: 469 us for the first.)
 #include "kin_chunk.h"
 
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(256 * RW, 2 * RW) void attention_mass_kernel(MassPa
       q = (int)((uint32_t)x * magic >> 16);
       g = x - q * p.group;
     };
-    // Stage `st`: 64 rows, swizzled; rows that do not count lie outside the descriptor's 1 GiB and read as zeros.
+    // Stage `st`: kMassRows rows, swizzled; rows that do not count lie outside the descriptor's 1 GiB and read as zeros.
     auto stage_rows = [&](int st) {
       const int r0 = first + st * kMassRows;
       const int i = r0 / p.group, g0 = r0 - i * p.group;

@@ -1048,7 +1048,8 @@ def qkv_norm_rope_split(qkv, q_weight, k_weight, eps: float, positions, freq, ax
     ``v[tokens, Hkv, D]`` from the fused projection, the q and k heads RMS-normalised (weights None: not) and their
     pairs (i, i + D/2) turned by ``positions[axis[i]] * frequency[i]``
     (the rotation of LiteSys/litesys/models/model_utils.py:17-52).  ``positions``: int32 [axes, tokens], or [tokens] for one axis;
-    ``freq``, ``axis``: ``rope_table``.  Angles are exact for every int32 position; one rounding at the end."""
+    ``freq``, ``axis``: ``rope_table``.  Position times stored fraction is taken modulo a turn exactly and then rounded to fp32, 2^-25.9 of
+    a turn off at most; the fraction itself is a float64 frequency, good to 2^-53 of it.  One rounding at the end."""
     tokens, width, stride = _row_view(qkv, "qkv")
     dev, dt = qkv.device, qkv.dtype
     _require(freq, "freq", torch.int64, 1, dev)
